@@ -344,6 +344,129 @@ int exl3_rope_append_fp8(void *qkv, int ld_qkv, const void *cos, const void *sin
                          float v_scale, void *stream);
 
 /*
+ * A paged KV cache of one layer, as the entry points below read and write it: page pools of equal layout for K and V;
+ * the element of (page p, head h, token t, dimension d) lies at p*page_stride + h*head_stride + t*token_stride + d
+ * (elements), which covers [pages][heads][page_size][head_dim] and [pages][page_size][heads][head_dim]; a contiguous
+ * cache [batch][heads][capacity][head_dim] is a pool of one page per sequence.  head_dim 128 or 256; strides
+ * multiples of 8 elements (16 for e4m3), pointers 16-byte aligned.  e4m3 caches hold value / scale (one positive
+ * scale per tensor); for the 16-bit types the scales are 1.
+ */
+enum { EXL3_KV_F16 = 0, EXL3_KV_BF16 = 1, EXL3_KV_E4M3 = 2 };
+typedef struct exl3_paged_cache {
+    void *k_pages, *v_pages;
+    long long page_stride, head_stride, token_stride;
+    int num_pages, page_size, kv_heads, head_dim;
+    int dtype;
+    float k_scale, v_scale;
+} exl3_paged_cache;
+
+/*
+ * Norms of the query and key heads, rotary embedding and the append to a paged cache in one pass, for any number of
+ * tokens, each at its own position (what exl3_rope_append is for one token per sequence, all at one position of a
+ * contiguous cache).  No counterpart in the reference: the serving engine does it there.
+ *   qkv       [tokens][ld_qkv] fp16 (bf16 when is_bf16): q_heads, then kv_heads key heads, then kv_heads value heads;
+ *             not modified, except the query heads when q_out is NULL (they are then rewritten in place)
+ *   q_out     [tokens][ld_q_out] (q_heads * head_dim values per row used), or NULL
+ *   norm      non-zero: every query and key head is multiplied by rsqrt(mean(x^2) + eps) and by q_weight / k_weight
+ *             ([head_dim], the type of qkv; NULL = ones) before it is rotated
+ *   cos, sin  fp32 [max_pos][rot_dim / 2]; rot_dim a multiple of 16, 0 = no rotation; dimensions from rot_dim on are
+ *             not rotated.  interleaved 0: pairs (i, i + rot_dim / 2), else (2 i, 2 i + 1)
+ *   positions, slots   int64 [tokens].  slot = page * page_size + offset; a token whose slot lies outside the pool
+ *             (-1 for padding) is not appended, its query is computed all the same.  A token whose position lies
+ *             outside the tables is left as it is altogether.  Two tokens must not have the same slot.
+ * fp32 arithmetic, one rounding: to the type of qkv, or (value / scale, saturating) to e4m3.
+ */
+int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out, long long ld_q_out, const void *q_weight,
+                             const void *k_weight, int norm, float eps, const void *cos, const void *sin, int rot_dim,
+                             int interleaved, int max_pos, const void *positions, const void *slots, int tokens,
+                             int q_heads, int is_bf16, const exl3_paged_cache *cache, void *stream);
+
+/*
+ * Attention of a tree of drafted tokens over a paged cache: several query tokens per sequence,
+ *     out[i][h][:] = softmax over the visible tokens t of (q[i][h] . K[t][h / G] * scale) . V[t][h / G],
+ * where the drafts of sequence b are the rows starts[b] .. starts[b+1]-1 of q, the n of them lie in the cache as its
+ * last n tokens (seq_lens counts them), and draft i sees every token before the drafts and those drafts j whose bit j
+ * is set in mask[i] (its ancestors and itself, in a tree); without a mask it sees the drafts up to itself.  A row
+ * that sees nothing yields zeros.  One token per sequence is ordinary decode attention.
+ *   q, out       [tokens][q_heads][head_dim] fp16 (bf16 when is_bf16), rows q_stride / out_stride elements apart
+ *                (multiples of 8), 16-byte aligned; rows at or behind starts[batch] are neither read nor written
+ *   block_table  int32 [batch][table_stride], table_width entries of a row used: the page of tokens i*page_size ..;
+ *                tokens on a page number outside the pool are not visible, entries behind a sequence's length are
+ *                not read
+ *   seq_lens     int32 [batch], drafts included; starts int32 [batch + 1], ascending; mask int64 [tokens] or NULL
+ *   max_drafts   1 .. EXL3_TREE_MAX_DRAFTS, the largest number of drafts of a sequence; rows of a sequence from
+ *                max_drafts on are not computed
+ *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads
+ *   workspace    exl3_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, need not be cleared; calls that share it
+ *                must not overlap on the device
+ * K and V are read at 16 bits (e4m3 widened exactly), scores, statistics and sums are fp32, the probabilities are
+ * rounded to the type of q before the product with V, the output once.  What lies in tokens that no row sees (NaN
+ * included) does not matter, nor what lies in a draft to the rows that do not see it.
+ */
+#define EXL3_TREE_MAX_DRAFTS 64
+size_t exl3_tree_attn_workspace_bytes(int batch, int q_heads, int max_drafts, const exl3_paged_cache *cache);
+int exl3_tree_attn(const void *q, long long q_stride, void *out, long long out_stride, const void *block_table,
+                   int table_stride, int table_width, const void *seq_lens, const void *starts, const void *mask,
+                   int batch, int tokens, int max_drafts, int q_heads, float scale, int is_bf16,
+                   const exl3_paged_cache *cache, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Pages of the caches, managed on the device: nothing returns to the host, so the calls take part in CUDA graphs.
+ * The state is in the caller's int32 arrays:
+ *   block_table [max_seqs][table_stride], seq_lens [max_seqs] (tokens), held [max_seqs] (pages of a sequence),
+ *   refs [num_pages] (sequences that hold a page), free_list [num_pages] (a stack of page numbers), counters [2] =
+ *   {pages on the stack, status bits}.  At the start: seq_lens, held, refs zero, free_list every page, counters
+ *   {num_pages, 0}.
+ * Lists of sequence numbers (int32, device memory) have at most EXL3_PAGES_MAX_SEQS entries.  The result is the one
+ * of serving the entries in their order, except that once the stack is too short for one, none behind it takes pages.
+ * An entry that cannot be served leaves its sequence as it was and sets a status bit (sticky; the caller reads and
+ * clears it when it likes): EXL3_PAGES_EXHAUSTED when the stack has too few pages, EXL3_PAGES_BAD when an index, a
+ * length or the state does not allow it (a sequence twice in a call, ...).
+ * Data is moved in all pools of `exl3_page_pools` (K and V of every layer: equal layouts, strides and row size in
+ * bytes, multiples of 16; page p of a pool and page p of another belong together).
+ */
+#define EXL3_PAGES_MAX_SEQS 1024
+#define EXL3_PAGES_MAX_POOLS 256
+enum { EXL3_PAGES_EXHAUSTED = 1, EXL3_PAGES_BAD = 2 };
+typedef struct exl3_page_tables {
+    void *block_table, *seq_lens, *held, *refs, *free_list, *counters;
+    int table_stride, table_width, max_seqs, num_pages, page_size;
+} exl3_page_tables;
+typedef struct exl3_page_pools {
+    void *const *pools;                 /* host array of num_pools device pointers */
+    long long page_stride, head_stride, token_stride;    /* bytes */
+    int num_pools, heads, row_bytes;    /* row_bytes: one token of one head, at most 1024 */
+} exl3_page_pools;
+/*
+ * children[i] (which hold nothing) become copies of parents[i]: full pages are shared, the used rows of a partial last
+ * page are copied to a page of their own.  A parent may have several children; it cannot be a child in the same call.
+ * workspace: exl3_cache_fork_workspace_bytes(n) bytes, 16-byte aligned, not shared by overlapping calls.
+ */
+size_t exl3_cache_fork_workspace_bytes(int n);
+int exl3_cache_fork(const exl3_page_pools *pools, const exl3_page_tables *tables, const void *parents,
+                    const void *children, int n, void *workspace, size_t workspace_bytes, void *stream);
+/*
+ * counts[i] more tokens for seqs[i]: pages as needed, seq_lens raised.  Outputs: base int32 [n] (the lengths before),
+ * starts int32 [n + 1] (prefix sums of counts), and for the tokens, one sequence after the other, slots and positions
+ * int64 [tokens] (what exl3_qk_norm_rope_append takes).  Tokens of a sequence that is not served, and entries behind
+ * the last token, have slot -1 (the latter position 0).  tokens: room in the outputs, at most 2^20; a sequence that
+ * does not fit is not served.  n >= 1.
+ */
+int exl3_cache_reserve(const exl3_page_tables *tables, const void *seqs, const void *counts, int n, void *slots,
+                       void *positions, int tokens, void *starts, void *base, void *stream);
+/*
+ * After a tree of drafts[i] tokens behind base[i] was verified: the rows at base + path[i][j], j < taken[i] (at most
+ * `most`, path is int32 [n][path_stride]), move to base + j in all pools, and seq_lens[seqs[i]] = base + taken.  The
+ * pages stay with the sequence.  The rows are moved as if all were read before the first is written; pages that are
+ * written must not be shared.
+ */
+int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_tables *tables, const void *seqs, const void *base,
+                      const void *drafts, const void *path, int path_stride, int most, const void *taken, int n,
+                      void *stream);
+/* The sequences give up their pages; those that no sequence holds any more return to the stack. */
+int exl3_cache_free(const exl3_page_tables *tables, const void *seqs, int n, void *stream);
+
+/*
  * Measurement probe (no counterpart in the reference, not on the layer's path): the rate at which the GPU can
  * decode the 3INST codebook with this library's decode routines and consume the codewords with mma.sync, on every
  * SM.  mode 0: words never leave registers (the ceiling the integer decode sets for any kernel of this design);

@@ -104,6 +104,25 @@ def lib():
                 L.exl3_decode_attn_paged_fp8.restype = ci
                 L.exl3_rope_append_fp8.argtypes = [vp, ci, vp, vp, ci, vp, vp, ci, ci, ci, ci, ci, ll, ll, cf, cf, vp]
                 L.exl3_rope_append_fp8.restype = ci
+                pc = ctypes.POINTER(Exl3PagedCache)
+                pt, pp = ctypes.POINTER(Exl3PageTables), ctypes.POINTER(Exl3PagePools)
+                L.exl3_qk_norm_rope_append.argtypes = [vp, ll, vp, ll, vp, vp, ci, cf, vp, vp, ci, ci, ci, vp, vp, ci, ci,
+                                                       ci, pc, vp]
+                L.exl3_qk_norm_rope_append.restype = ci
+                L.exl3_tree_attn_workspace_bytes.restype = sz
+                L.exl3_tree_attn_workspace_bytes.argtypes = [ci, ci, ci, pc]
+                L.exl3_tree_attn.argtypes = [vp, ll, vp, ll, vp, ci, ci, vp, vp, vp, ci, ci, ci, ci, cf, ci, pc, vp, sz, vp]
+                L.exl3_tree_attn.restype = ci
+                L.exl3_cache_fork_workspace_bytes.restype = sz
+                L.exl3_cache_fork_workspace_bytes.argtypes = [ci]
+                L.exl3_cache_fork.argtypes = [pp, pt, vp, vp, ci, vp, sz, vp]
+                L.exl3_cache_fork.restype = ci
+                L.exl3_cache_reserve.argtypes = [pt, vp, vp, ci, vp, vp, ci, vp, vp, vp]
+                L.exl3_cache_reserve.restype = ci
+                L.exl3_cache_accept.argtypes = [pp, pt, vp, vp, vp, vp, ci, ci, vp, ci, vp]
+                L.exl3_cache_accept.restype = ci
+                L.exl3_cache_free.argtypes = [pt, vp, ci, vp]
+                L.exl3_cache_free.restype = ci
                 for name in ("exl3_reconstruct", "exl3_had_r_128", "exl3_gemv_grouped", "exl3_gemv",
                              "exl3_int8_embed", "exl3_int8_head"):
                     getattr(L, name).restype = ci
@@ -588,3 +607,301 @@ def decode_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Ten
     else:
         _check(L.exl3_decode_attn_paged(*args, _stream(q)), "exl3_decode_attn_paged")
     return out
+
+
+# --------------------------------------------------------------------------- paged caches: append, tree attention, pages
+class Exl3PagedCache(ctypes.Structure):
+    _fields_ = [("k_pages", ctypes.c_void_p), ("v_pages", ctypes.c_void_p), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong), ("num_pages", ctypes.c_int),
+                ("page_size", ctypes.c_int), ("kv_heads", ctypes.c_int), ("head_dim", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("k_scale", ctypes.c_float), ("v_scale", ctypes.c_float)]
+
+
+class Exl3PageTables(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("block_table", "seq_lens", "held", "refs", "free_list", "counters")] + \
+               [(n, ctypes.c_int) for n in ("table_stride", "table_width", "max_seqs", "num_pages", "page_size")]
+
+
+class Exl3PagePools(ctypes.Structure):
+    _fields_ = [("pools", ctypes.POINTER(ctypes.c_void_p)), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong), ("num_pools", ctypes.c_int),
+                ("heads", ctypes.c_int), ("row_bytes", ctypes.c_int)]
+
+
+TREE_MAX_DRAFTS = 64
+PAGES_MAX_SEQS = 1024
+PAGES_MAX_POOLS = 256
+PAGES_EXHAUSTED, PAGES_BAD = 1, 2
+_KV_KIND = {torch.float16: 0, torch.bfloat16: 1, FP8: 2}
+
+
+def _need(ok: bool, what: str):
+    if not ok:
+        raise RuntimeError(what)
+
+
+def _call(dev: torch.device, fn, *args):
+    """fn(*args, stream): the current stream of `dev`, with `dev` current while it launches."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _check(rc, fn.__name__)
+
+
+def _ints(t, name: str, dev: torch.device, dtype=torch.int32, dim: int = 1):
+    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype or t.dim() != dim or \
+            (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise RuntimeError(f"{name} must be a {dim}-D {dtype} tensor on {dev} with contiguous rows")
+    return t
+
+
+def _paged(name: str, x: torch.Tensor, k, v, layout: str, k_scale: float, v_scale: float) -> Exl3PagedCache:
+    """The description of the page pools that the C entry points take; x holds the 16-bit values beside them."""
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
+        raise RuntimeError(f"{name}: CUDA tensors are needed (this build has no CPU path)")
+    if x.dtype not in _DT or k.dtype != v.dtype or k.dtype not in (x.dtype, FP8):
+        raise RuntimeError(f"{name}: fp16 or bf16 values, and page pools both of that type or both float8_e4m3fn")
+    if layout not in ("HND", "NHD") or k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1 \
+            or k.device != x.device or v.device != x.device:
+        raise RuntimeError(f"{name}: page pools must be 4-D on the device of the values, with equal shapes and strides, "
+                           "layout HND or NHD")
+    if k.dtype != FP8 and (k_scale != 1.0 or v_scale != 1.0):
+        raise RuntimeError(f"{name}: scales belong to float8_e4m3fn page pools")
+    shape, stride = k.shape, k.stride()
+    h, t = (1, 2) if layout == "HND" else (2, 1)
+    # a size-one dimension has no stride of its own
+    ts = stride[t] if shape[t] > 1 else (shape[3] if layout == "HND" else shape[2] * shape[3])
+    hs = stride[h] if shape[h] > 1 else (ts * shape[t] if layout == "HND" else shape[3])
+    ps = stride[0] if shape[0] > 1 else ts * shape[t] + hs * shape[h]
+    return Exl3PagedCache(k.data_ptr(), v.data_ptr(), ps, hs, ts, shape[0], shape[t], shape[h], shape[3],
+                          _KV_KIND[k.dtype], k_scale, v_scale)
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, positions: torch.Tensor,
+                        slots: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, q_heads: int,
+                        q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                        eps: float | None = 1e-6, interleaved: bool = False, layout: str = "HND",
+                        q_out: torch.Tensor | None = None, k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+    """Norms of the query and key heads, rotary embedding and the append to a paged cache, one pass over
+    qkv [T, >= (q_heads + 2 kv_heads) * hd] (fp16 or bf16, contiguous rows; hd 128 or 256).
+
+    Every query and key head is normed (x * rsqrt(mean(x^2) + eps) * weight; eps None: not, weight None: ones) and
+    rotated by row positions[t] of cos, sin (fp32 [max_pos, rot / 2], rot a multiple of 16; None: not rotated; pairs
+    (i, i + rot/2), or (2i, 2i + 1) when interleaved).  Keys and values go to slots[t] = page * page_size + offset of
+    the page pools (see decode_attn_paged; any page size), as value / scale in float8_e4m3fn ones; a slot outside the
+    pool (-1 for padding) is skipped.  A token whose position is outside the tables is left as it is.  positions and
+    slots are int64 [T]; no two tokens may share a slot.  The queries go to q_out [T, q_heads, hd], or back to their
+    place in qkv; returns them."""
+    cache = _paged("qk_norm_rope_append", qkv, k_pages, v_pages, layout, k_scale, v_scale)
+    dev, hd = qkv.device, cache.head_dim
+    _need(qkv.dim() == 2 and (qkv.stride(1) == 1) and q_heads > 0 and qkv.shape[1] >= (q_heads + 2 * cache.kv_heads) * hd,
+          "qk_norm_rope_append: qkv must be [T, (q_heads + 2 kv_heads) * hd] with contiguous rows")
+    T = qkv.shape[0]
+    _ints(positions, "positions", dev, torch.int64)
+    _ints(slots, "slots", dev, torch.int64)
+    _need(positions.shape[0] == T and slots.shape[0] == T, "qk_norm_rope_append: positions and slots must be [T]")
+    rot, rows = 0, 1
+    _need((cos is None) == (sin is None), "qk_norm_rope_append: cos and sin belong together")
+    if cos is not None:
+        _cuda(cos, "cos", torch.float32)
+        _cuda(sin, "sin", torch.float32)
+        _need(cos.dim() == 2 and cos.shape == sin.shape and cos.device == dev and sin.device == dev,
+              "qk_norm_rope_append: cos and sin must be [max_pos, rot / 2] on the device of qkv")
+        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    else:
+        rows = 2 ** 31 - 1                                # no table: no position is outside of it
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _cuda(w, name, qkv.dtype)
+            _need(w.shape == (hd,) and w.device == dev, f"{name} must be [hd] on the device of qkv")
+    ldq = 0
+    if q_out is not None:
+        _need(isinstance(q_out, torch.Tensor) and q_out.device == dev and q_out.dtype == qkv.dtype and
+              q_out.shape == (T, q_heads, hd) and q_out.stride(2) == 1 and (q_heads == 1 or q_out.stride(1) == hd),
+              "qk_norm_rope_append: q_out must be [T, q_heads, hd] in the type of qkv, with contiguous heads")
+        ldq = q_out.stride(0) if T > 1 else q_heads * hd
+    if T == 0:
+        return q_out if q_out is not None else torch.as_strided(qkv, (0, q_heads, hd), (qkv.stride(0), hd, 1))
+    ld = qkv.stride(0) if T > 1 else -(-qkv.shape[1] // 8) * 8
+    _call(dev, lib().exl3_qk_norm_rope_append, qkv.data_ptr(), ld, None if q_out is None else q_out.data_ptr(), ldq,
+          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+          0 if eps is None else 1, 0.0 if eps is None else eps, None if cos is None else cos.data_ptr(),
+          None if sin is None else sin.data_ptr(), rot, 1 if interleaved else 0, rows, positions.data_ptr(),
+          slots.data_ptr(), T, q_heads, 1 if qkv.dtype == torch.bfloat16 else 0, ctypes.byref(cache))
+    return q_out if q_out is not None else torch.as_strided(qkv, (T, q_heads, hd), (qkv.stride(0), hd, 1))
+
+
+def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
+                    seq_lens: torch.Tensor, starts: torch.Tensor, max_drafts: int, tree_mask: torch.Tensor | None = None,
+                    layout: str = "HND", scale: float | None = None, out: torch.Tensor | None = None,
+                    k_scale: float = 1.0, v_scale: float = 1.0) -> torch.Tensor:
+    """decode_attn_paged for a tree of drafted tokens per sequence: softmax(q K^T * scale) V over the visible tokens.
+
+    q [T, q_heads, hd] fp16 or bf16 (contiguous heads, hd 128 or 256): sequence b's drafts are rows starts[b] ..
+    starts[b+1]-1 (int32 [B + 1]), at most max_drafts (1 .. 64) of them, and lie in the cache as its last tokens
+    (seq_lens, int32 [B], counts them).  Draft i sees the tokens before the drafts and those drafts j of its sequence
+    whose bit j is set in tree_mask[row] (int64 [T]: its ancestors and itself; None: every draft up to itself).  A row
+    that sees nothing gives zeros.  Page pools and block_table as for decode_attn_paged (q's type or float8_e4m3fn; page
+    size a multiple of 16); tokens on a page number outside the pool are not visible.  Rows of q from starts[B] on are
+    not read, those of `out` not written.  Returns [T, q_heads, hd] in q's type."""
+    cache = _paged("tree_attn_paged", q, k_pages, v_pages, layout, k_scale, v_scale)
+    dev, hd = q.device, cache.head_dim
+    _need(q.dim() == 3 and q.shape[2] == hd and q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == hd),
+          "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
+    T, qh = q.shape[0], q.shape[1]
+    _ints(block_table, "block_table", dev, torch.int32, 2)
+    _ints(seq_lens, "seq_lens", dev)
+    _ints(starts, "starts", dev)
+    B = block_table.shape[0]
+    _need(seq_lens.shape[0] == B and starts.shape[0] == B + 1, "tree_attn_paged: seq_lens must be [B], starts [B + 1]")
+    if tree_mask is not None:
+        _ints(tree_mask, "tree_mask", dev, torch.int64)
+        _need(tree_mask.shape[0] == T, "tree_attn_paged: tree_mask must be [T]")
+    if out is None:
+        out = torch.empty((T, qh, hd), dtype=q.dtype, device=dev)
+    else:
+        _need(isinstance(out, torch.Tensor) and out.device == dev and out.dtype == q.dtype and out.shape == q.shape and
+              out.stride(2) == 1 and (qh == 1 or out.stride(1) == hd),
+              "tree_attn_paged: out must be [T, heads, hd] in the type of q, with contiguous heads")
+    if T == 0 or B == 0:
+        _need(1 <= max_drafts <= TREE_MAX_DRAFTS and qh > 0 and qh % cache.kv_heads == 0, "tree_attn_paged: bad max_drafts or heads")
+        return out
+    L, row = lib(), qh * hd
+    cref = ctypes.byref(cache)
+    need = L.exl3_tree_attn_workspace_bytes(B, qh, max_drafts, cref)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _call(dev, L.exl3_tree_attn, q.data_ptr(), q.stride(0) if T > 1 else row, out.data_ptr(), out.stride(0) if T > 1 else row,
+          block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], block_table.shape[1],
+          seq_lens.data_ptr(), starts.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), B, T, max_drafts, qh,
+          hd ** -0.5 if scale is None else scale, 1 if q.dtype == torch.bfloat16 else 0, cref,
+          None if ws is None else ws.data_ptr(), need)
+    return out
+
+
+def page_tables(max_seqs: int, pages_per_seq: int, num_pages: int, device) -> dict:
+    """The state of an empty set of sequences over `num_pages` pages, as the cache_* calls take it (int32 tensors):
+    block_table [max_seqs, pages_per_seq], seq_lens (tokens), held (pages) [max_seqs], refs [num_pages] (sequences that
+    hold a page), free_list (a stack), counters [2] = pages on the stack, status bits (PAGES_EXHAUSTED, PAGES_BAD)."""
+    def zeros(*n):
+        return torch.zeros(n, dtype=torch.int32, device=device)
+    return dict(block_table=zeros(max_seqs, pages_per_seq), seq_lens=zeros(max_seqs), held=zeros(max_seqs),
+                refs=zeros(num_pages), free_list=torch.arange(num_pages - 1, -1, -1, dtype=torch.int32, device=device),
+                counters=torch.tensor([num_pages, 0], dtype=torch.int32, device=device))
+
+
+def _tables(tables: dict, page_size: int):
+    bt, lens, held, refs, free, cnt = (tables[n] for n in ("block_table", "seq_lens", "held", "refs", "free_list", "counters"))
+    if not isinstance(bt, torch.Tensor) or bt.device.type != "cuda":
+        raise RuntimeError("block_table must be a CUDA tensor (this build has no CPU path)")
+    dev = bt.device
+    _ints(bt, "block_table", dev, torch.int32, 2)
+    for t, name in ((lens, "seq_lens"), (held, "held"), (refs, "refs"), (free, "free_list"), (cnt, "counters")):
+        _ints(t, name, dev)
+    S, P, N = bt.shape[0], bt.shape[1], refs.shape[0]
+    _need(lens.shape[0] == S and held.shape[0] == S and free.shape[0] == N and cnt.shape[0] == 2,
+          "page tables: seq_lens and held must be [max_seqs], free_list [num_pages], counters [2]")
+    return dev, Exl3PageTables(bt.data_ptr(), lens.data_ptr(), held.data_ptr(), refs.data_ptr(), free.data_ptr(),
+                               cnt.data_ptr(), bt.stride(0) if S > 1 else P, P, S, N, page_size)
+
+
+def _pools(pools, layout: str, dev: torch.device, num_pages: int):
+    """The page pools of all layers: one tensor [n, pages, ...] or a sequence of equal pools."""
+    if isinstance(pools, torch.Tensor):
+        _need(pools.dim() == 5 and pools.device == dev, "pools must be [n, pages, ...] on the device of the tables, or a list of pools")
+        n, shape, stride = pools.shape[0], pools.shape[1:], pools.stride()[1:]
+        size = pools.element_size()
+        base, step = pools.data_ptr(), pools.stride(0) * size
+        where = [base + i * step for i in range(n)]
+    else:
+        n = len(pools)
+        _need(n > 0 and all(isinstance(p, torch.Tensor) and p.device == dev and p.dim() == 4 for p in pools),
+              "pools must be 4-D tensors on the device of the tables")
+        shape, stride, size = pools[0].shape, pools[0].stride(), pools[0].element_size()
+        _need(all(p.shape == shape and p.stride() == stride and p.dtype == pools[0].dtype for p in pools),
+              "pools must have equal shapes, strides and types")
+        where = [p.data_ptr() for p in pools]
+    _need(len(set(where)) == n, "pools must be different pools")
+    ptrs = (ctypes.c_void_p * max(n, 1))(*where)
+    _need(layout in ("HND", "NHD") and stride[3] == 1, "pools: layout HND or NHD, contiguous rows")
+    _need(shape[0] == num_pages, "pools must have as many pages as the tables count")
+    h, t = (1, 2) if layout == "HND" else (2, 1)
+    ts = stride[t] if shape[t] > 1 else (shape[3] if layout == "HND" else shape[2] * shape[3])
+    hs = stride[h] if shape[h] > 1 else (ts * shape[t] if layout == "HND" else shape[3])
+    ps = stride[0] if shape[0] > 1 else ts * shape[t] + hs * shape[h]
+    return shape[t], Exl3PagePools(ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p)), ps * size, hs * size, ts * size, n,
+                                   shape[h], shape[3] * size)
+
+
+def _page_size(pools, layout: str) -> int:
+    first = pools if isinstance(pools, torch.Tensor) else (pools[0] if len(pools) else None)
+    _need(isinstance(first, torch.Tensor) and first.dim() >= 4, "pools must be page pools")
+    return first.shape[-2] if layout == "HND" else first.shape[-3]
+
+
+def cache_fork(pools, tables: dict, parents: torch.Tensor, children: torch.Tensor, layout: str = "HND") -> None:
+    """Make sequences children[i] (which hold nothing) copies of parents[i] (int32 [n], n <= 1024): full pages are
+    shared, the used rows of a partial last page are copied to a new page in every pool.  pools: the K and V page
+    pools of all layers, one tensor [n_pools, pages, ...] or a list of equal pools (at most 256); tables: page_tables()."""
+    dev, tab = _tables(tables, _page_size(pools, layout))
+    _, pl = _pools(pools, layout, dev, tab.num_pages)
+    _ints(parents, "parents", dev)
+    _ints(children, "children", dev)
+    n = parents.shape[0]
+    _need(children.shape[0] == n, "cache_fork: as many children as parents")
+    if n == 0:
+        return
+    L = lib()
+    need = L.exl3_cache_fork_workspace_bytes(n)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    _call(dev, L.exl3_cache_fork, ctypes.byref(pl), ctypes.byref(tab), parents.data_ptr(), children.data_ptr(), n,
+          None if ws is None else ws.data_ptr(), need)
+
+
+def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_size: int, tokens: int):
+    """Room for counts[i] more tokens of sequence seqs[i] (int32 [n], 1 <= n <= 1024): takes pages as needed and raises
+    seq_lens.  Returns (slots [tokens], positions [tokens], starts [n + 1], base [n]): where each new token goes and its
+    position, one sequence after the other, the sequences' first rows (what qk_norm_rope_append and tree_attn_paged
+    take), and the lengths before.  Slots behind the last token, and those of a sequence that could not be served
+    (counters[1]), are -1."""
+    dev, tab = _tables(tables, page_size)
+    _ints(seqs, "seqs", dev)
+    _ints(counts, "counts", dev)
+    n = seqs.shape[0]
+    _need(counts.shape[0] == n and n > 0 and tokens >= 0, "cache_reserve: seqs and counts must be [n], n > 0")
+    where = torch.empty((2, tokens), dtype=torch.int64, device=dev)
+    rows = torch.empty((2 * n + 1,), dtype=torch.int32, device=dev)
+    slots, positions, starts, base = where[0], where[1], rows[:n + 1], rows[n + 1:]
+    _call(dev, lib().exl3_cache_reserve, ctypes.byref(tab), seqs.data_ptr(), counts.data_ptr(), n, slots.data_ptr(),
+          positions.data_ptr(), tokens, starts.data_ptr(), base.data_ptr())
+    return slots, positions, starts, base
+
+
+def cache_accept(pools, tables: dict, seqs: torch.Tensor, base: torch.Tensor, drafts: torch.Tensor, path: torch.Tensor,
+                 taken: torch.Tensor, layout: str = "HND") -> None:
+    """After drafts[i] drafted tokens behind base[i] of sequence seqs[i] were verified: move the rows of the accepted
+    drafts path[i, :taken[i]] (int32 [n, most], most <= 64) to base[i], base[i] + 1, .. in every pool, and set seq_lens
+    to base + taken.  Pages stay with the sequence.  pools, tables: as for cache_fork."""
+    dev, tab = _tables(tables, _page_size(pools, layout))
+    _, pl = _pools(pools, layout, dev, tab.num_pages)
+    for t, name in ((seqs, "seqs"), (base, "base"), (drafts, "drafts"), (taken, "taken")):
+        _ints(t, name, dev)
+    _ints(path, "path", dev, torch.int32, 2)
+    n, most = path.shape
+    _need(seqs.shape[0] == n and base.shape[0] == n and drafts.shape[0] == n and taken.shape[0] == n,
+          "cache_accept: seqs, base, drafts and taken must be [n], path [n, most]")
+    if n == 0:
+        return
+    _call(dev, lib().exl3_cache_accept, ctypes.byref(pl), ctypes.byref(tab), seqs.data_ptr(), base.data_ptr(),
+          drafts.data_ptr(), path.data_ptr(), path.stride(0) if n > 1 else most, most, taken.data_ptr(), n)
+
+
+def cache_free(tables: dict, seqs: torch.Tensor) -> None:
+    """Give up the pages of the sequences seqs (int32 [n], n <= 1024); those that nobody holds any more are free again."""
+    dev, tab = _tables(tables, 1)
+    _ints(seqs, "seqs", dev)
+    if seqs.shape[0] == 0:
+        return
+    _call(dev, lib().exl3_cache_free, ctypes.byref(tab), seqs.data_ptr(), seqs.shape[0])
