@@ -396,7 +396,7 @@ int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out, long long
  *   seq_lens     int32 [batch], drafts included; starts int32 [batch + 1], ascending; mask int64 [tokens] or NULL
  *   max_drafts   1 .. EXL3_TREE_MAX_DRAFTS, the largest number of drafts of a sequence; rows of a sequence from
  *                max_drafts on are not computed
- *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads
+ *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads, at most 64 times as many
  *   workspace    exl3_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, need not be cleared; calls that share it
  *                must not overlap on the device
  * K and V are read at 16 bits (e4m3 widened exactly), scores, statistics and sums are fp32, the probabilities are
@@ -409,6 +409,11 @@ int exl3_tree_attn(const void *q, long long q_stride, void *out, long long out_s
                    int table_stride, int table_width, const void *seq_lens, const void *starts, const void *mask,
                    int batch, int tokens, int max_drafts, int q_heads, float scale, int is_bf16,
                    const exl3_paged_cache *cache, void *workspace, size_t workspace_bytes, void *stream);
+/* Sticky status word of exl3_tree_attn's bounded waits on the current device (0 = none ran out; waits for the device),
+ * its reset, and the self-test of the wait as for exl3_gemm_tc. */
+int exl3_tree_attn_status(unsigned *status_out);
+int exl3_tree_attn_status_reset(void);
+int exl3_tree_attn_selftest_wait(unsigned limit_us, void *stream);
 
 /*
  * Pages of the caches, managed on the device: nothing returns to the host, so the calls take part in CUDA graphs.

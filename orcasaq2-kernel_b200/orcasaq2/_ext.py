@@ -113,6 +113,11 @@ def lib():
                 L.exl3_tree_attn_workspace_bytes.argtypes = [ci, ci, ci, pc]
                 L.exl3_tree_attn.argtypes = [vp, ll, vp, ll, vp, ci, ci, vp, vp, vp, ci, ci, ci, ci, cf, ci, pc, vp, sz, vp]
                 L.exl3_tree_attn.restype = ci
+                L.exl3_tree_attn_status.argtypes = [ctypes.POINTER(ctypes.c_uint)]
+                L.exl3_tree_attn_status.restype = ci
+                L.exl3_tree_attn_status_reset.restype = ci
+                L.exl3_tree_attn_selftest_wait.argtypes = [ctypes.c_uint, vp]
+                L.exl3_tree_attn_selftest_wait.restype = ci
                 L.exl3_cache_fork_workspace_bytes.restype = sz
                 L.exl3_cache_fork_workspace_bytes.argtypes = [ci]
                 L.exl3_cache_fork.argtypes = [pp, pt, vp, vp, ci, vp, sz, vp]
@@ -779,6 +784,14 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
           hd ** -0.5 if scale is None else scale, 1 if q.dtype == torch.bfloat16 else 0, cref,
           None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def tree_attn_status(device: torch.device) -> int:
+    """Sticky status word of tree_attn_paged's bounded waits on `device` (0 = healthy)."""
+    word = ctypes.c_uint(0)
+    with torch.cuda.device(device):
+        _check(lib().exl3_tree_attn_status(ctypes.byref(word)), "exl3_tree_attn_status")
+    return int(word.value)
 
 
 def page_tables(max_seqs: int, pages_per_seq: int, num_pages: int, device) -> dict:
