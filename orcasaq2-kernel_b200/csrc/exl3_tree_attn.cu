@@ -5,28 +5,29 @@
 //     S[row][token] = Q (shared memory) x K^T (shared memory, K-major)          fp32 in tensor memory
 //     P = exp2(S * scale - m), rounded to 16 bits, in place of S                tensor memory
 //     O[row][dim]  += P (tensor memory) x V (shared memory, MN-major: V lies [token][dim] as the cache has it)
-// A row's statistics are one thread's: its TMEM lane holds all 128 scores of the block, no shuffles.
+// Two threads share a row (a TMEM lane), 64 scores of the block each, held in registers: no shuffles, one exchange of
+// the maximum through shared memory.
 //
 // What bounds it: K and V are read once per 128 rows, 4 * HD * 128 * 128 multiply-adds for 4 * HD * 128 bytes; at 128
 // rows the tensor cores need a third of the time that HBM takes, so up to 128 rows the kernel's business is to keep
-// loads in flight: a ring of 32 KB stages (128 tokens x 128 dimensions of K or of V) filled by TMA boxes of 8 tokens
-// (eight rows of a swizzle atom; a page is a multiple of them), all boxes of a stage issued by one instruction of
-// sixteen lanes.  More rows are more tiles: CTAs of the tiles of one sequence walk the same blocks at the same time
-// and share them in L2.
+// loads in flight: a ring of 32 KB stages (128 tokens x 128 dimensions of K, 64 x 256 or 128 x 128 of V), filled by four
+// warps with 16-byte cp.async straight into the swizzled places, each thread's arrival on the stage's barrier following
+// its copies.  (TMA boxes were measured first: pages allow boxes of 8 or 16 tokens only, and sixteen 2 KB boxes took
+// 1700 cycles a stage, whether the bytes came from HBM or from L2.)  More rows are more tiles: CTAs of the tiles of one
+// sequence walk the same blocks at the same time and share them in L2.
 // Work is split evenly whatever the lengths: the blocks of all (sequence, KV head) pairs form one line, every CTA
 // takes an equal piece of it (found from the lengths on the device), and a pair that several CTAs share leaves partial
 // sums with their maximum, which a second kernel joins in order (fixed order: the same bytes every run).
 // The running maximum is only raised when it grows by more than 8 (a factor of 256 that the fp32 sums and the 16-bit
 // probabilities hold easily), so O is seldom rescaled.
 //
-// Tokens nobody sees must not matter, whatever they hold: box rows behind the end and rows on pages outside the pool
-// come in as zeros (TMA fill of an out-of-range page), the rest of the last box is zeroed, and non-finite V values of
-// drafts, which some rows see and others do not, are zeroed before the product and added to the rows that see them at
-// the end (a path that finite caches never take).
+// Tokens nobody sees must not matter, whatever they hold: rows behind the end and rows on pages outside the pool are
+// filled with zeros instead of read, and non-finite V values of drafts, which some rows see and others do not, are
+// zeroed before the product and added to the rows that see them at the end (a path that finite caches never take).
 //
-// e4m3 caches: raw stages, eight converter warps widen them exactly to the 16-bit type of q into the same swizzled
-// stages; the scales fold into the softmax scale and the normalisation.
-#include <cuda.h>
+// e4m3 caches: the four warps fetch 16 KB raw stages, every thread its own pieces (so it waits for nobody else's), and
+// widen them exactly to the 16-bit type of q into the swizzled stages; the scales fold into the softmax scale and the
+// normalisation.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -50,7 +51,6 @@ constexpr int kStageBytes = kTok * kDims * 2; // 32 KB
 constexpr int kRawBytes = kTok * kDims;       // 16 KB of e4m3
 constexpr int kMaxTiles = 32;
 constexpr int kMaxGrid = 148;
-constexpr int kConvWarps = 8;
 constexpr float kRaise = 8.f;                 // log2 units the maximum may lag behind
 
 static __device__ unsigned g_tree_status;     // sticky: non-zero after a bounded wait ran out
@@ -59,18 +59,30 @@ struct Params {
     const void *q;
     void *out;
     long long q_stride, out_stride;
-    const void *v;                            // for the non-finite path only
+    const void *k, *v;
     long long page_stride, head_stride, tok_stride;
     const int *block_table, *seq_lens, *starts;
     const long long *mask;
     int bt_stride, width, num_pages, page_size;
     int batch, tokens, max_drafts, kvh, G, tiles;    // tiles: of the sequence with the most drafts
     float scale_log2, v_scale;
-    int negate;                               // the scale is negative: q is negated, scale_log2 is its size
-    int rows_ws;                              // rows of a partial result
+    int negate;                               // the scale is negative: Q K^T is negated, scale_log2 is its size
+    int rows_ws;                              // rows of a partial result (a multiple of 32)
     int *plan;                                // [0..32) CTAs per tile, [32..64) blocks per tile, then per tile [batch + 1] prefix sums
-    float *part_ml, *part_o;                  // [2 * grid][rows_ws][2], [2 * grid][rows_ws][HD]
+    float *part_ml, *part_o;                  // [2 * grid][2][rows_ws], [2 * grid][HD / 4][rows_ws][4]: lane = row, full lines
 };
+
+struct Shared {
+    uint64_t full[6], empty[6];
+    uint64_t s_full[2], p_ready[2], v_here[2], pv_done[2], q_full, q_empty, o_free, drain;
+    uint32_t tmem_base;
+    int nonfinite[2];                         // of the current segment and the one before, in turn
+    float top[2][2][kM];                      // maxima of the two halves of a row, two blocks
+    int total[kMaxTiles];
+    int sums[16];                             // one per warp
+    int first_seq, first_off;
+};
+static_assert(sizeof(Shared) <= 3072, "shared state");
 
 template <bool FP8, int HD>
 struct Cfg {
@@ -78,30 +90,18 @@ struct Cfg {
     static constexpr int kQBytes = kM * HD * 2;
     static constexpr int kStages = FP8 ? 3 : (HD == 256 ? 5 : 6);
     static constexpr int kRaw = FP8 ? 4 : 0;
-    static constexpr int kThreads = FP8 ? 256 + 32 * kConvWarps : 256;
-    static constexpr int kSmem = kQBytes + kStages * kStageBytes + kRaw * kRawBytes + 1024 /*barriers*/ + 1024 /*alignment*/;
+    static constexpr int kThreads = 512;          // 1 MMA + 3 query + 8 softmax + 4 fetch warps
+    static constexpr int kSmem = kQBytes + kStages * kStageBytes + kRaw * kRawBytes + sizeof(Shared);
 };
 
-struct Shared {
-    uint64_t full[6], empty[6], raw_full[4], raw_empty[4];
-    uint64_t s_full[2], p_ready[2], v_here[2], pv_done[2], q_full, q_empty, o_free, drain;
-    uint32_t tmem_base;
-    int nonfinite;
-    int total[kMaxTiles];
-    int sums[16];
-    int first_seq, first_off;
-};
-static_assert(sizeof(Shared) <= 1024, "shared state");
 
-__device__ __forceinline__ void tma_5d(uint32_t dst, const CUtensorMap *map, int a, int b, int c, int d, int e, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-        ::"r"(dst), "l"(map), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e), "r"(bar) : "memory");
+// Sixteen bytes into shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void tma_4d(uint32_t dst, const CUtensorMap *map, int a, int b, int c, int d, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(map), "r"(a), "r"(b), "r"(c), "r"(d), "r"(bar) : "memory");
+// This thread's arrival on the barrier once its copies so far have landed.
+__device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 // Shared-memory operand, 128-byte swizzle.  K-major: rows of 128 bytes, groups of eight rows `sbo` bytes apart.
 // MN-major: atoms of 64 values x 8 k, `lbo` bytes apart along the values, `sbo` along k.
@@ -125,8 +125,8 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
           "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -136,19 +136,29 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
           "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
           "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-          "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
-}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// The two warps of a quarter of the rows; all eight softmax warps.
+__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+// Two fp32 operations at a time.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 
 // ---------------------------------------------------------------- the line of blocks
 struct Seq { int first, n, len, rows, blocks; };    // first row of q, drafts, tokens, query rows per KV head, blocks
@@ -195,33 +205,47 @@ struct Walk {
     __device__ __forceinline__ int rows() const { return min(kM, s.rows - kM * m); }
 };
 
-// CTAs of a tile out of `grid`, in proportion to its blocks (at least one).  Tiles of equal work get equal numbers, so
-// that their CTAs walk the same blocks at the same time.  One thread; U[m] falls with m.
-__device__ __forceinline__ int share_out(const int *U, int tiles, int grid, int m_wanted, int *m_of, int cta) {
-    long long all = 0;
-    for (int m = 0; m < tiles; ++m) all += U[m];
-    int used = 0, first = 0;
-    for (int m = 0; m < tiles; ++m) used += U[m] ? max(1, (int)((long long)grid * U[m] / all)) : 0;
-    int at = 0;
-    *m_of = -1;
-    for (int m = 0; m < tiles; ++m) {
-        int w = U[m] ? max(1, (int)((long long)grid * U[m] / all)) : 0;
-        if (m == 0) w -= max(0, used - grid);
-        if (m == m_wanted) first = at;
-        if (cta >= at && cta < at + w) { *m_of = m; first = at; m_wanted = m; }
-        at += w;
+// CTAs of tile `lane` out of `grid`, in proportion to its blocks (at least one).  Tiles of equal work get equal numbers,
+// so that their CTAs walk the same blocks at the same time.  A whole warp; totals[0] is the largest.
+__device__ __forceinline__ int share_of(const int *totals, int tiles, int grid, int lane) {
+    if (tiles == 1) return lane == 0 && totals[0] ? grid : 0;
+    const double u = lane < tiles ? totals[lane] : 0;
+    double all = u;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    int w = u > 0 ? max(1, (int)(grid * u / all)) : 0;
+    const int used = __reduce_add_sync(0xffffffffu, w);
+    if (lane == 0) w -= max(0, used - grid);
+    return w;
+}
+// First block of piece w when U blocks are cut into W pieces.
+__device__ __forceinline__ int piece(int U, int W, int w) {
+    const int q = U / W;
+    return w * q + min(w, U - q * W);
+}
+
+// The pages of the sixteen-token (or shorter) pieces at t, t + 128, t + 256 .. of a sequence, one lookup ahead.
+struct PageCursor {
+    const int *row;                    // of the block table
+    int t, len, idx, at, size, step_idx, step_at, num_pages, ahead;
+    __device__ __forceinline__ void begin(const Params &P, int b, int tok, int length) {
+        row = P.block_table + (size_t)b * P.bt_stride;
+        t = tok; len = length; size = P.page_size; num_pages = P.num_pages;
+        idx = t / size; at = t - idx * size;
+        step_idx = kTok / size; step_at = kTok - step_idx * size;
+        ahead = t < len ? __ldg(row + idx) : -1;
     }
-    return first;
-}
-__device__ __forceinline__ int share_of(const int *U, int tiles, int grid, int m) {
-    long long all = 0;
-    int used = 0;
-    for (int i = 0; i < tiles; ++i) all += U[i];
-    for (int i = 0; i < tiles; ++i) used += U[i] ? max(1, (int)((long long)grid * U[i] / all)) : 0;
-    const int w = U[m] ? max(1, (int)((long long)grid * U[m] / all)) : 0;
-    return m == 0 ? w - max(0, used - grid) : w;
-}
-__device__ __forceinline__ int cut(int U, int W, int w) { return (int)((long long)U * w / W); }
+    // (page, token in the page) of the current piece, page -1 when none of it is there; then on to the next
+    __device__ __forceinline__ int take(int &in_page, int &tokens) {
+        const int page = (unsigned)ahead < (unsigned)num_pages ? ahead : -1;
+        in_page = at;
+        tokens = page < 0 ? 0 : len - t;
+        t += kTok; idx += step_idx; at += step_at;
+        if (at >= size) { at -= size; ++idx; }
+        ahead = t < len ? __ldg(row + idx) : -1;
+        return page;
+    }
+};
 
 // ---------------------------------------------------------------- e4m3 -> 16 bits
 template <typename T>
@@ -244,25 +268,26 @@ __device__ __forceinline__ bool nonfinite2(uint32_t w, uint32_t &keep) {      //
 
 template <typename T, bool FP8, int HD>
 __global__ void __launch_bounds__(Cfg<FP8, HD>::kThreads, 1)
-tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const __grid_constant__ Params P) {
+tree_attn_kernel(const __grid_constant__ Params P) {
     using C = Cfg<FP8, HD>;
     constexpr int H = C::kHalves;
     constexpr int kThreads = C::kThreads;
-    constexpr int kBox = FP8 ? 16 : 8;                       // tokens of a TMA box
-    extern __shared__ unsigned char smem_dyn[];
-    unsigned char *const smem = smem_dyn + ((1024u - (s32(smem_dyn) & 1023u)) & 1023u);
+    extern __shared__ __align__(1024) unsigned char smem[];      // (swizzle atoms are 1 KB)
     unsigned char *const smQ = smem, *const ring = smQ + C::kQBytes, *const rawring = ring + C::kStages * kStageBytes;
     Shared &S = *reinterpret_cast<Shared *>(rawring + C::kRaw * kRawBytes);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned *const status = &g_tree_status;
+    if (s32(smem) & 1023u) {
+        if (tid == 0) atomicOr(status, 2u);
+        return;
+    }
 
     if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.full[i]), FP8 ? kConvWarps : 1); mbar_init(s32(&S.empty[i]), 1); }
-        for (int i = 0; i < C::kRaw; ++i) { mbar_init(s32(&S.raw_full[i]), 1); mbar_init(s32(&S.raw_empty[i]), kConvWarps); }
-        for (int i = 0; i < 2; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 4); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
-        mbar_init(s32(&S.q_full), 2); mbar_init(s32(&S.q_empty), 1);
-        mbar_init(s32(&S.o_free), 4); mbar_init(s32(&S.drain), 1);
-        S.nonfinite = 0;
+        for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.full[i]), FP8 ? 4 : 128); mbar_init(s32(&S.empty[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 8); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
+        mbar_init(s32(&S.q_full), 96); mbar_init(s32(&S.q_empty), 1);
+        mbar_init(s32(&S.o_free), 8); mbar_init(s32(&S.drain), 1);
+        S.nonfinite[0] = S.nonfinite[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
@@ -286,18 +311,23 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
         }
     }
     __syncthreads();
-    int m;
-    const int cta0 = share_out(S.total, P.tiles, gridDim.x, -1, &m, blockIdx.x);
-    int u0 = 0, u1 = 0, w = 0;
-    if (m >= 0) {
-        w = blockIdx.x - cta0;
-        const int W = share_of(S.total, P.tiles, gridDim.x, m);
-        u0 = cut(S.total[m], W, w);
-        u1 = cut(S.total[m], W, w + 1);
-        if (w == 0 && tid == 0) { P.plan[m] = W; P.plan[kMaxTiles + m] = S.total[m]; }
+    int m = 0, w = blockIdx.x, W = 0;
+    {
+        const int mine = share_of(S.total, P.tiles, gridDim.x, lane);
+        int upto = mine;                                     // CTAs of the tiles up to this lane's
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const uint32_t behind = __ballot_sync(0xffffffffu, upto > (int)blockIdx.x);
+        m = behind ? __ffs(behind) - 1 : 0;
+        W = __shfl_sync(0xffffffffu, behind ? mine : 0, m);
+        w -= __shfl_sync(0xffffffffu, upto - mine, m);
+        if (blockIdx.x == 0 && tid < P.tiles) { P.plan[tid] = mine; P.plan[kMaxTiles + tid] = S.total[tid]; }
     }
-    if (blockIdx.x == 0 && tid < P.tiles && S.total[tid] == 0) { P.plan[tid] = 0; P.plan[kMaxTiles + tid] = 0; }
-    if (m >= 0 && (u1 > u0 || w == 0)) {
+    const int u0 = W ? piece(S.total[m], W, w) : 0, u1 = W ? piece(S.total[m], W, w + 1) : 0;
+    if (W && (u1 > u0 || w == 0)) {
         int carry = 0;
         for (int b0 = 0; b0 < P.batch; b0 += kThreads) {
             const int b = b0 + tid;
@@ -309,7 +339,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 const int y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= o) x += y;
             }
-            __syncthreads();
+            if (b0) __syncthreads();
             if (lane == 31) S.sums[warp] = x;
             __syncthreads();
             int before = carry, all = 0;
@@ -328,57 +358,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
 
     if (u1 > u0) {
         Walk wk(P, m, S.first_seq, S.first_off, u1 - u0);
-        if (warp == 0) {
-            // ---------------- producer: lane g fetches boxes of eight tokens (e4m3: sixteen)
-            constexpr int kBoxes = kTok / kBox;
-            constexpr int kSlots = FP8 ? C::kRaw : C::kStages;
-            constexpr uint32_t kBytes = FP8 ? kRawBytes : kStageBytes;
-            uint64_t *const full = FP8 ? S.raw_full : S.full, *const empty = FP8 ? S.raw_empty : S.empty;
-            unsigned char *const slots = FP8 ? rawring : ring;
-            Cursor rc(0, kSlots);
-            int filled = 0;
-            bool ok = true;
-            const auto page_of = [&](int tok0) {           // this lane's page, or one outside the pool
-                const int t = tok0 + (lane % kBoxes) * kBox;
-                if (t >= wk.s.len) return P.num_pages;
-                const int page = __ldg(P.block_table + (size_t)wk.b * P.bt_stride + t / P.page_size);
-                return page >= 0 && page < P.num_pages ? page : P.num_pages;
-            };
-            const auto fetch = [&](const CUtensorMap *map, int tok0, int page) {
-                for (int h = 0; h < H && ok; ++h, rc.advance(1), ++filled) {
-                    if (lane == 0 && rc.wrapped) ok = mbar_wait(s32(&empty[rc.idx]), rc.phase ^ 1u, status, 20);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const uint32_t bar = s32(&full[rc.idx]);
-                    if (lane == 0) mbar_expect_tx(bar, kBytes);
-                    __syncwarp();
-                    if (lane < kBoxes) {
-                        const uint32_t dst = s32(slots + (size_t)rc.idx * kBytes) + lane * (kBytes / kBoxes);
-                        const int at = (tok0 + lane * kBox) % P.page_size;
-                        if constexpr (FP8) tma_4d(dst, map, h * kDims, at, wk.hk, page, bar);
-                        else tma_5d(dst, map, 0, at, 2 * h, wk.hk, page, bar);
-                    }
-                }
-            };
-            while (ok && wk.next()) {
-                const int t0 = wk.blk * kTok;
-                int page = page_of(t0);
-                fetch(&kmap, t0, page);
-                for (int i = 0; i < wk.nb && ok; ++i) {
-                    const int tok0 = t0 + i * kTok, ahead = i + 1 < wk.nb ? page_of(tok0 + kTok) : P.num_pages;
-                    if (i + 1 < wk.nb) fetch(&kmap, tok0 + kTok, ahead);
-                    fetch(&vmap, tok0, page);
-                    page = ahead;
-                }
-            }
-            // every copy issued has landed before the CTA goes (they have, unless a wait ran out)
-            if (lane == 0)
-                for (int f = max(0, filled - kSlots); f < filled; ++f) mbar_wait(s32(&full[f % kSlots]), (f / kSlots) & 1, status, 20);
-        } else if (warp == 1) {
+        if (warp == 1) {
             // ---------------- the MMAs
             if (lane == 0) {
                 constexpr uint32_t kType = __is_same(T, __half) ? 0u : (1u << 7 | 1u << 10);
-                const uint32_t id_qk = umma_idesc_f16(kM, kTok) | kType, id_pv = umma_idesc_f16(kM, kDims) | kType | 1u << 16;
+                const uint32_t id_qk = umma_idesc_f16(kM, kTok) | kType | (P.negate ? 1u << 13 : 0u);      // bit 13: -A
+                const uint32_t id_pv = umma_idesc_f16(kM, HD) | kType | 1u << 16;                          // bit 16: B is MN-major
                 Cursor rc(0, C::kStages);
                 bool ok = true;
                 int cnt = 0;                                   // blocks whose probabilities were used
@@ -387,6 +372,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     for (int h = 0; h < H && ok; ++h, rc.advance(1)) {
                         ok = mbar_wait(s32(&S.full[rc.idx]), rc.phase, status);
                         if (!ok) return;
+                        if constexpr (!FP8) fence_async();     // the copies were the other warps', plain ones
                         fence_after_sync();
                         const uint32_t kb = s32(ring + (size_t)rc.idx * kStageBytes);
 #pragma unroll
@@ -400,6 +386,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                 while (ok && wk.next()) {
                     ok = mbar_wait(s32(&S.q_full), wk.index & 1, status);
                     if (!ok) break;
+                    fence_async();
                     fence_after_sync();
                     scores(cnt);
                     if (wk.nb == 1) umma_commit(s32(&S.q_empty));
@@ -414,13 +401,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                         if (ok) ok = mbar_wait(s32(&S.p_ready[cnt & 1]), (cnt >> 1) & 1, status);
                         if (ok && i == 0 && wk.index) ok = mbar_wait(s32(&S.o_free), (wk.index - 1) & 1, status);
                         if (!ok) break;
+                        if constexpr (!FP8) fence_async();
                         fence_after_sync();
                         for (int h = 0; h < H; ++h, rc.advance(1)) {
                             const uint32_t vb = s32(ring + (size_t)rc.idx * kStageBytes);
-                            const uint32_t p = tmem + HD + (cnt & 1) * kTok;
+                            const uint32_t p = tmem + HD + (cnt & 1) * kTok + h * (kTok / H / 2);
 #pragma unroll
-                            for (int k = 0; k < kTok / 16; ++k)
-                                umma_f16_ts(tmem + h * kDims, p + 8 * k, desc_sw128(vb + k * 4096, 1024, 2048), id_pv, i || k);
+                            for (int k = 0; k < kTok / H / 16; ++k)
+                                umma_f16_ts(tmem, p + 8 * k, desc_sw128(vb + k * (HD * 32), 1024, HD * 16), id_pv, i || h || k);
                             umma_commit(s32(&S.empty[rc.idx]));
                         }
                         umma_commit(s32(&S.pv_done[cnt & 1]));
@@ -431,61 +419,71 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
             }
         } else if (warp < 4) {
             // ---------------- query rows into shared memory (swizzled, K-major), rows behind the last one zero
+            constexpr int kUnits = HD / 8, kRows = 32 / kUnits;   // 16-byte units of a row, rows of an instruction
             bool ok = true;
-            constexpr int kUnits = HD / 8;                     // 16-byte units of a row
+            const int u = lane % kUnits, sub = lane / kUnits;
+            int filled = kM;                                   // rows that may hold something
             while (ok && wk.next()) {
                 if (wk.index) {
-                    ok = mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status, 20);
+                    ok = mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
-                const int rows = wk.rows();
-                const uint32_t flip = P.negate ? 0x80008000u : 0u;
-                for (int e = (warp - 2) * 32 + lane; e < kM * kUnits; e += 64) {
-                    const int r = e / kUnits, u = e - r * kUnits, c = u >> 3;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (r < rows) {
-                        const int R = kM * m + r, i = R / P.G, g = R - i * P.G;
-                        x = *reinterpret_cast<const uint4 *>(static_cast<const T *>(P.q) + (size_t)(wk.s.first + i) * P.q_stride +
-                                                             (size_t)(wk.hk * P.G + g) * HD + 8 * u);
-                        x.x ^= flip; x.y ^= flip; x.z ^= flip; x.w ^= flip;
-                    }
-                    *reinterpret_cast<uint4 *>(smQ + c * (kM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = x;
+                const int rows = wk.rows(), upto = max(filled, rows);
+                constexpr int kStep = 3 * kRows;
+                int r = (warp ? warp - 1 : 0) * kRows + sub, i = (kM * m + r) / P.G, g = kM * m + r - i * P.G;
+                const T *const base = static_cast<const T *>(P.q) + (size_t)wk.s.first * P.q_stride + (size_t)wk.hk * P.G * HD + 8 * u;
+                const uint32_t dst = s32(smQ) + (u >> 3) * (kM * 128);
+                const int di = kStep / P.G, dg = kStep - di * P.G;
+#pragma unroll 4
+                for (; r < rows; r += kStep) {
+                    copy16(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4), base + i * P.q_stride + g * HD, true);
+                    i += di; g += dg;
+                    if (g >= P.G) { g -= P.G; ++i; }
                 }
+                for (; r < upto; r += kStep)
+                    *reinterpret_cast<uint4 *>(smQ + (u >> 3) * (kM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
                 fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s32(&S.q_full));
+                filled = rows;
+                arrive_behind_copies(s32(&S.q_full));
             }
-        } else if (warp < 8) {
-            // ---------------- softmax: thread = row = TMEM lane
-            const int row = tid - 128;
-            const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else if (warp < 12) {
+            // ---------------- softmax: a thread has 64 scores of its row (TMEM lane)
+            const int quarter = warp & 3, row = 32 * quarter + lane, side = (warp - 4) >> 2;
+            const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
+            constexpr int kCols = HD / 2;                      // of O, this thread's half
+            const uint32_t o_t = tmem + lane_base + side * kCols;
+            // These warps meet at barriers: after a wait that ran out they walk on without waiting (what they write is
+            // garbage then, the status word says so).
             bool ok = true;
+            const auto hold = [&](uint64_t *bar, uint32_t parity) {
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s32(bar), parity, status));
+                fence_after_sync();
+            };
             int cnt = 0, pos = 0;                              // blocks done; ring position of the segment
-            while (ok && wk.next()) {
+            while (wk.next()) {
+                const int rows = wk.rows();
                 const int R = kM * m + row, draft = R / P.G;
-                const bool live = row < wk.rows();
+                const bool live = row < rows;
                 const int ctx = wk.s.len - wk.s.n;             // first draft's token (negative: drafts that have none)
                 unsigned long long bits = 0;
                 if (live) bits = P.mask ? (unsigned long long)__ldg(P.mask + wk.s.first + draft) : (draft >= 63 ? ~0ull : (2ull << draft) - 1);
-                float top = -INFINITY, sum = 0.f;
-                const auto page_ok = [&](int tok0) {           // lanes 0..15: is the page of eight tokens in the pool?
-                    const int t = tok0 + (lane & 15) * 8;
-                    if (t >= wk.s.len) return true;
-                    const int page = __ldg(P.block_table + (size_t)wk.b * P.bt_stride + t / P.page_size);
-                    return page >= 0 && page < P.num_pages;
-                };
-                bool pages = page_ok(wk.blk * kTok);
-                for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
+                float top = -INFINITY;
+                float2 sum2 = make_float2(0.f, 0.f);           // of this thread's columns
+                PageCursor pc;                                 // lanes 0..3: sixteen tokens of this half each
+                pc.begin(P, wk.b, wk.blk * kTok + 64 * side + 16 * (lane & 3), wk.s.len);
+                for (int i = 0; i < wk.nb; ++i, ++cnt) {
                     const int tok0 = (wk.blk + i) * kTok;
-                    const uint32_t groups = __ballot_sync(0xffffffffu, pages) & 0xFFFFu;
-                    if (i + 1 < wk.nb) pages = page_ok(tok0 + kTok);
-                    const bool masked = tok0 + kTok > ctx || groups != 0xFFFFu;        // uniform in the four warps
-                    uint32_t vis[4] = {~0u, ~0u, ~0u, ~0u};
+                    int in_page, there;
+                    pc.take(in_page, there);
+                    const uint32_t groups = __ballot_sync(0xffffffffu, there > 0) & 0xFu;
+                    const bool masked = tok0 + kTok > ctx || groups != 0xFu;           // uniform in the warp
+                    uint32_t vis[2] = {~0u, ~0u};
                     if (masked) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const int a = tok0 + 32 * k;
+                        for (int k = 0; k < 2; ++k) {
+                            const int a = tok0 + 64 * side + 32 * k;
                             uint32_t v = 0;
                             // context tokens of these 32, then the drafts' bits shifted to their places
                             const int c = ctx - a, l = wk.s.len - a;
@@ -493,88 +491,83 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                             else if (c > 0) v = (1u << c) - 1 | (uint32_t)(bits << c);
                             else v = -c < 64 ? (uint32_t)(bits >> -c) : 0u;
                             if (l < 32) v &= l > 0 ? (1u << l) - 1 : 0u;
-                            const uint32_t g4 = groups >> (4 * k) & 15u;
-                            v &= (g4 & 1 ? 0xFFu : 0u) | (g4 & 2 ? 0xFF00u : 0u) | (g4 & 4 ? 0xFF0000u : 0u) | (g4 & 8 ? 0xFF000000u : 0u);
+                            v &= (groups >> (2 * k) & 1 ? 0xFFFFu : 0u) | (groups >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
                             vis[k] = live ? v : 0u;
                         }
                     }
                     const uint32_t s_t = tmem + lane_base + HD + (cnt & 1) * kTok;
-                    ok = __all_sync(0xffffffffu, mbar_wait(s32(&S.s_full[cnt & 1]), (cnt >> 1) & 1, status));
-                    if (!ok) break;
-                    fence_after_sync();
+                    hold(&S.s_full[cnt & 1], (cnt >> 1) & 1);
+                    uint32_t x[2][32];
+                    tmem_ld32(s_t + 64 * side, x[0]);
+                    tmem_ld32(s_t + 64 * side + 32, x[1]);
+                    tmem_wait_ld();
                     float mx = -INFINITY;
+                    if (masked) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t x[32];
-                        tmem_ld32(s_t + 32 * k, x);
-                        if (masked) {
+                        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, vis[e >> 5] >> (e & 31) & 1 ? __uint_as_float(x[e >> 5][e & 31]) : -INFINITY);
+                    } else {
+                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, vis[k] >> e & 1 ? __uint_as_float(x[e]) : -INFINITY);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(x[e]));
-                        }
+                        for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(x[e >> 5][e & 31]));
+                        mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     }
+                    S.top[cnt & 1][side][row] = mx;
+                    fence_before_sync();
+                    pair_sync(quarter);                        // (after which both halves' scores are in registers, too)
+                    fence_after_sync();
+                    mx = fmaxf(mx, S.top[cnt & 1][side ^ 1][row]);
                     mx = mx == -INFINITY ? mx : mx * P.scale_log2;
                     const bool raise = mx > top + kRaise || (top == -INFINITY && mx > top);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float corr = raise ? ex2(top - mx) : 1.f;      // 0 when nothing was seen before
-                        if (raise) { top = mx; sum *= corr; }
+                        if (raise) { top = mx; sum2.x *= corr; sum2.y *= corr; }
                         if (i > 0) {
-                            ok = __all_sync(0xffffffffu, mbar_wait(s32(&S.pv_done[(cnt - 1) & 1]), ((cnt - 1) >> 1) & 1, status));
-                            if (!ok) break;
-                            fence_after_sync();
-#pragma unroll
-                            for (int c = 0; c < HD; c += 32) {
+                            hold(&S.pv_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1);
+#pragma unroll 1
+                            for (int c = 0; c < kCols; c += 32) {
                                 uint32_t o[32];
-                                tmem_ld32(tmem + lane_base + c, o);
+                                tmem_ld32(o_t + c, o);
+                                tmem_wait_ld();
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st32(tmem + lane_base + c, o);
+                                tmem_st32(o_t + c, o);
                             }
                         }
                     }
                     const float shift = top == -INFINITY ? 0.f : top;
+                    const float2 mul = make_float2(P.scale_log2, P.scale_log2), sub = make_float2(-shift, -shift);
+                    uint32_t p[32];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t x[32], p[16];
-                        tmem_ld32(s_t + 32 * k, x);
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float a = ex2(fmaf(__uint_as_float(x[2 * e]), P.scale_log2, -shift));
-                            float c = ex2(fmaf(__uint_as_float(x[2 * e + 1]), P.scale_log2, -shift));
-                            if (masked) {
-                                if (!(vis[k] >> (2 * e) & 1)) a = 0.f;
-                                if (!(vis[k] >> (2 * e + 1) & 1)) c = 0.f;
-                            }
-                            sum += a + c;
-                            p[e] = Type16<T>::pack(a, c);
+                    for (int e = 0; e < 32; ++e) {
+                        const int k = e >> 4, c = 2 * (e & 15);
+                        float2 a = fma2(make_float2(__uint_as_float(x[k][c]), __uint_as_float(x[k][c + 1])), mul, sub);
+                        a.x = ex2(a.x);
+                        a.y = ex2(a.y);
+                        if (masked) {
+                            if (!(vis[k] >> c & 1)) a.x = 0.f;
+                            if (!(vis[k] >> (c + 1) & 1)) a.y = 0.f;
                         }
-                        tmem_st16(s_t + 16 * k, p);            // over scores that were read
+                        sum2 = add2(sum2, a);
+                        p[e] = Type16<T>::pack(a.x, a.y);
                     }
+                    tmem_st32(s_t + 32 * side, p);             // over scores that both threads have read
                     if (tok0 + kTok > ctx) {
-                        // rows of V behind the end become zeros, non-finite values of drafts too (see the top of the file)
-                        const int from = max(0, ctx - tok0), have = min(kTok, wk.s.len - tok0), upto = min(kTok, (have + kBox - 1) & ~(kBox - 1));
+                        // non-finite values of drafts become zeros (see the top of the file)
+                        const int from = max(0, ctx - tok0), upto = min(kTok, wk.s.len - tok0);
                         const int vpos = pos + H + 2 * H * i + (i + 1 < wk.nb ? H : 0);
                         // (announced by the MMA thread, which looks at every stage in its turn: the stage's own barrier may
                         // still be a whole round behind, or ahead, of what this thread would wait for)
-                        ok = __all_sync(0xffffffffu, mbar_wait(s32(&S.v_here[cnt & 1]), (cnt >> 1) & 1, status));
-                        if (!ok) break;
-                        for (int h = 0; h < H; ++h) {
-                            const int st = (vpos + h) % C::kStages;
-                            for (int e = row; e < (upto - from) * 16; e += 128) {
-                                const int r = from + (e >> 4), u = e & 15;
-                                uint4 *const at = reinterpret_cast<uint4 *>(ring + (size_t)st * kStageBytes + (r >> 3) * 2048 + (u >> 3) * 1024 +
-                                                                            (r & 7) * 128 + (((u & 7) ^ (r & 7)) << 4));
-                                if (r >= have) {
-                                    *at = make_uint4(0, 0, 0, 0);
-                                } else {
-                                    uint4 x = *at, y;
-                                    const bool a = nonfinite2<T>(x.x, y.x), b2 = nonfinite2<T>(x.y, y.y), c = nonfinite2<T>(x.z, y.z),
-                                               d = nonfinite2<T>(x.w, y.w);
-                                    if (a || b2 || c || d) { *at = y; S.nonfinite = 1; }
-                                }
-                            }
+                        hold(&S.v_here[cnt & 1], (cnt >> 1) & 1);
+                        constexpr int kUnits = HD / 8, kRowsV = kTok / H;           // 16-byte units of a row, rows of a stage
+                        for (int e = tid - 128; e < (upto - from) * kUnits; e += 256) {
+                            const int r = from + e / kUnits, u = e % kUnits, st = (vpos + r / kRowsV) % C::kStages, q = r % kRowsV;
+                            uint4 *const at = reinterpret_cast<uint4 *>(ring + (size_t)st * kStageBytes + (q >> 3) * (HD * 16) + (u >> 3) * 1024 +
+                                                                        (q & 7) * 128 + (((u & 7) ^ (q & 7)) << 4));
+                            const uint4 v = *at;
+                            uint4 y;
+                            const bool a = nonfinite2<T>(v.x, y.x), b2 = nonfinite2<T>(v.y, y.y), c = nonfinite2<T>(v.z, y.z),
+                                       d = nonfinite2<T>(v.w, y.w);
+                            if (a || b2 || c || d) { *at = y; S.nonfinite[wk.index & 1] = 1; }
                         }
                         fence_async();
                     }
@@ -583,99 +576,288 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
                     __syncwarp();
                     if (lane == 0) mbar_arrive(s32(&S.p_ready[cnt & 1]));
                 }
-                if (!ok) break;
                 // ---- the segment's result
-                ok = __all_sync(0xffffffffu, mbar_wait(s32(&S.pv_done[(cnt - 1) & 1]), ((cnt - 1) >> 1) & 1, status));
-                if (!ok) break;
-                fence_after_sync();
+                float sum = sum2.x + sum2.y;
+                S.top[cnt & 1][side][row] = sum;               // (the buffer of the block before last: read by all)
+                hold(&S.pv_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1);
                 softmax_sync();
-                const bool mend = S.nonfinite != 0;            // uniform: all have written it before the barrier
+                sum = S.top[cnt & 1][0][row] + S.top[cnt & 1][1][row];
+                const bool mend = S.nonfinite[wk.index & 1] != 0;       // uniform: all have written it before the barrier
+                if (tid == 128) S.nonfinite[wk.index & 1 ^ 1] = 0;      // read before the last barrier, written behind the next
                 const bool whole = wk.whole();
                 const float inv = sum == 0.f ? 0.f : P.v_scale / sum;
                 const int slot = 2 * blockIdx.x + (wk.index ? 1 : 0);
-                T *const orow = static_cast<T *>(P.out) + (size_t)(wk.s.first + draft) * P.out_stride + (size_t)(wk.hk * P.G + R - draft * P.G) * HD;
-                float *const prow = P.part_o + ((size_t)slot * P.rows_ws + row) * HD;
+                float4 *const pcol = reinterpret_cast<float4 *>(P.part_o) + ((size_t)slot * (HD / 4) + side * (kCols / 4)) * P.rows_ws + row;
+                T *orow[4];                                    // rows 4 (lane / 4) + 0..3 of the quarter, this lane's sixteen bytes
+                if (whole) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 32 * quarter + (lane & 28) + k, Rk = kM * m + r, i = Rk / P.G;
+                        orow[k] = r < rows ? static_cast<T *>(P.out) + (size_t)(wk.s.first + i) * P.out_stride +
+                                                 (size_t)(wk.hk * P.G + Rk - i * P.G) * HD + side * kCols + 8 * (lane & 3) : nullptr;
+                    }
+                }
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
+                for (int c = 0; c < kCols; c += 32) {
                     uint32_t o[32];
-                    tmem_ld32(tmem + lane_base + c, o);
+                    tmem_ld32(o_t + c, o);
+                    tmem_wait_ld();
                     if (mend && live) {
                         const int t_end = min(wk.s.len, (wk.blk + wk.nb) * kTok);
                         for (int t = max(max(0, ctx), wk.blk * kTok); t < t_end; ++t) {
                             if (t - ctx > 63 || !(bits >> (t - ctx) & 1)) continue;
                             const int page = __ldg(P.block_table + (size_t)wk.b * P.bt_stride + t / P.page_size);
                             if (page < 0 || page >= P.num_pages) continue;
-                            const size_t at = (size_t)page * P.page_stride + (size_t)wk.hk * P.head_stride + (size_t)(t % P.page_size) * P.tok_stride + c;
+                            const size_t at = (size_t)page * P.page_stride + (size_t)wk.hk * P.head_stride +
+                                              (size_t)(t % P.page_size) * P.tok_stride + side * kCols + c;
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                float x;
-                                if constexpr (FP8) x = (float)static_cast<const __nv_fp8_e4m3 *>(P.v)[at + e];
-                                else x = (float)static_cast<const T *>(P.v)[at + e];
-                                if (!isfinite(x)) o[e] = __float_as_uint(__uint_as_float(o[e]) + x);
+                                float v;
+                                if constexpr (FP8) v = (float)static_cast<const __nv_fp8_e4m3 *>(P.v)[at + e];
+                                else v = (float)static_cast<const T *>(P.v)[at + e];
+                                if (!isfinite(v)) o[e] = __float_as_uint(__uint_as_float(o[e]) + v);
                             }
                         }
                     }
-                    if (live && whole) {
+                    __syncwarp();
+                    if (whole) {
+                        // a lane's 64 bytes are four pieces; four lanes exchange pieces so that each writes one piece of four
+                        // rows, 64 contiguous bytes of a row from four lanes (a lane's own row: a line per lane and store)
+                        uint32_t w[4][4];
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 r;
-                            r.x = Type16<T>::pack(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-                            r.y = Type16<T>::pack(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-                            r.z = Type16<T>::pack(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-                            r.w = Type16<T>::pack(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(orow + c + e) = r;
+                        for (int e = 0; e < 16; ++e)
+                            w[e >> 2][e & 3] = Type16<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+                            for (int q = 0; q < 4; q += 2) {
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & 1 ? w[q][k] : w[q + 1][k], 1);
+                                if (lane & 1) w[q][k] = got; else w[q + 1][k] = got;
+                            }
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & 2 ? w[q][k] : w[q + 2][k], 2);
+                                if (lane & 2) w[q][k] = got; else w[q + 2][k] = got;
+                            }
                         }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            if (orow[k]) *reinterpret_cast<uint4 *>(orow[k] + c) = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
                     } else if (live) {
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<uint4 *>(prow + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            pcol[(c + e) / 4 * P.rows_ws] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]),
+                                                                        __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3]));
                     }
                     __syncwarp();
                 }
-                if (live && !whole) *reinterpret_cast<float2 *>(P.part_ml + ((size_t)slot * P.rows_ws + row) * 2) = make_float2(top, sum);
+                if (live && !whole && side == 0) {
+                    P.part_ml[(size_t)(2 * slot) * P.rows_ws + row] = top;
+                    P.part_ml[(size_t)(2 * slot + 1) * P.rows_ws + row] = sum;
+                }
                 fence_before_sync();
-                softmax_sync();
-                if (row == 0) S.nonfinite = 0;
                 softmax_sync();
                 if (lane == 0) mbar_arrive(s32(&S.o_free));
                 pos += 2 * H * wk.nb;
             }
-        } else if constexpr (FP8) {
-            // ---------------- e4m3 stages -> 16-bit stages: sixteen bytes per thread and step, two units of the swizzled row
-            const int ct = tid - 256;
-            Cursor rc(0, C::kRaw), cc(0, C::kStages);
+        } else if constexpr (!FP8) {
+            // ---------------- cache rows into the ring: a warp takes sixteen tokens of either half of a block
+            const int fw = warp - 12;
+            Cursor rc(0, C::kStages);
             bool ok = true;
-            while (ok && wk.next()) {
-                for (int i = 0; i < 2 * H * wk.nb && ok; ++i, rc.advance(1), cc.advance(1)) {
-                    ok = mbar_wait(s32(&S.raw_full[rc.idx]), rc.phase, status, 20);
-                    if (ok && cc.wrapped) ok = mbar_wait(s32(&S.empty[cc.idx]), cc.phase ^ 1u, status, 20);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    const unsigned char *const src = rawring + (size_t)rc.idx * kRawBytes;
-                    unsigned char *const dst = ring + (size_t)cc.idx * kStageBytes;
-                    uint4 x[4];
+            // K stages (and V of 128 dimensions): an instruction is two rows of 256 bytes; V of 256 dimensions: one of 512
+            const int half = lane >> 4, uk = lane & 15;
+            uint32_t place_k[4], place_v[8];                   // inside a stage, rows 2 j + half, rows j
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4 *>(src + 16 * (ct + 256 * j));
+            for (int j = 0; j < 4; ++j) {
+                const int r = 2 * j + half;
+                place_k[j] = s32(ring) + fw * 4096 + (uk >> 3) * 1024 + r * 128 + (((uk & 7) ^ r) << 4);
+            }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int e = ct + 256 * j, r = e >> 3, u = e & 7;
-                        uint4 a, b;
-                        widen4<T>(x[j].x, a.x, a.y);
-                        widen4<T>(x[j].y, a.z, a.w);
-                        widen4<T>(x[j].z, b.x, b.y);
-                        widen4<T>(x[j].w, b.z, b.w);
-                        unsigned char *const at = dst + (r >> 3) * 2048 + (u >> 2) * 1024 + (r & 7) * 128;
-                        const int k = (u & 3) * 2;
-                        // the two halves of a row's lanes start with different units: no bank conflicts
-                        const bool swap = u & 4;
-                        *reinterpret_cast<uint4 *>(at + (((k + (swap ? 1 : 0)) ^ (r & 7)) << 4)) = swap ? b : a;
-                        *reinterpret_cast<uint4 *>(at + (((k + (swap ? 0 : 1)) ^ (r & 7)) << 4)) = swap ? a : b;
+            for (int j = 0; j < 8; ++j) place_v[j] = s32(ring) + fw * 8192 + (lane >> 3) * 1024 + j * 128 + (((lane & 7) ^ j) << 4);
+            PageCursor pc[2];                                  // of either half
+            long long off[2], noff[2] = {0, 0};                // elements from the pool to its first row
+            int rows[2], nrows[2] = {0, 0};                    // rows that are there
+            const auto locate = [&](long long (&o)[2], int (&n)[2]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    int at;
+                    const int page = pc[g].take(at, n[g]);
+                    o[g] = page < 0 ? 0ll : page * P.page_stride + wk.hk * P.head_stride + at * P.tok_stride;
+                }
+            };
+            const auto slot = [&]() {                          // the next stage is free
+                if (rc.wrapped) ok = mbar_wait(s32(&S.empty[rc.idx]), rc.phase ^ 1u, status);
+                ok = __all_sync(0xffffffffu, ok);
+                return ok;
+            };
+            const long long two = 2 * P.tok_stride;
+            const auto fetch_wide = [&](const void *pool, const long long (&o)[2], const int (&n)[2], int dim) {   // 128 tokens x 128 dims
+                if (!slot()) return;
+                const uint32_t stage = rc.idx * kStageBytes;
+                const T *const from = static_cast<const T *>(pool) + dim + 8 * uk + half * P.tok_stride;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const T *src = from + o[g];
+                    const bool all = n[g] >= 16;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j, src += two) {
+                        const uint32_t dst = place_k[j & 3] + stage + g * 16384 + (j >> 2) * 2048;
+                        const bool real = all || 2 * j + half < n[g];
+                        copy16(dst, real ? src : static_cast<const T *>(pool), real);
                     }
-                    fence_async();
-                    __syncwarp();
-                    if (lane == 0) { mbar_arrive(s32(&S.raw_empty[rc.idx])); mbar_arrive(s32(&S.full[cc.idx])); }
+                }
+                arrive_behind_copies(s32(&S.full[rc.idx]));
+                rc.advance(1);
+            };
+            const auto fetch_tall = [&](const void *pool, long long o, int n) {                                     // 64 tokens x 256 dims
+                if (!slot()) return;
+                const uint32_t stage = rc.idx * kStageBytes;
+                const T *src = static_cast<const T *>(pool) + o + 8 * lane;
+                const bool all = n >= 16;
+#pragma unroll
+                for (int j = 0; j < 16; ++j, src += P.tok_stride) {
+                    const bool real = all || j < n;
+                    copy16(place_v[j & 7] + stage + (j >> 3) * 4096, real ? src : static_cast<const T *>(pool), real);
+                }
+                arrive_behind_copies(s32(&S.full[rc.idx]));
+                rc.advance(1);
+            };
+            while (ok && wk.next()) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) pc[g].begin(P, wk.b, wk.blk * kTok + 64 * g + 16 * fw, wk.s.len);
+                locate(off, rows);
+                for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, off, rows, h * kDims);
+                for (int i = 0; i < wk.nb && ok; ++i) {
+                    if (i + 1 < wk.nb) {
+                        locate(noff, nrows);
+                        for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, noff, nrows, h * kDims);
+                    }
+                    if constexpr (H == 2) {
+                        for (int h = 0; h < 2 && ok; ++h) fetch_tall(P.v, off[h], rows[h]);
+                    } else if (ok) {
+                        fetch_wide(P.v, off, rows, 0);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) { off[g] = noff[g]; rows[g] = nrows[g]; }
                 }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            // ---------------- e4m3 rows: as above, into raw stages (a warp has 4 KB of one), in instructions of four rows of
+            // 128 bytes, or two of 256; what a thread fetched it widens itself, kRaw - 1 stages later, sixteen bytes into two
+            // units of the swizzled row
+            const int fw = warp - 12;
+            const uint32_t raw = s32(rawring) + fw * 4096 + 16 * lane;
+            const unsigned char *const rawp = rawring + fw * 4096 + 16 * lane;
+            Cursor cc(0, C::kStages);
+            bool ok = true;
+            int issued = 0, done = 0;
+            uint32_t tall = 0;                                 // bit s % kRaw: raw stage s is 64 tokens x 256 bytes
+            const auto widen = [&]() {
+                if (cc.wrapped) ok = mbar_wait(s32(&S.empty[cc.idx]), cc.phase ^ 1u, status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) return;
+                const int rs = done % C::kRaw;
+                const unsigned char *const src = rawp + rs * kRawBytes;
+                unsigned char *const dst = ring + cc.idx * kStageBytes;
+                const bool is_tall = H == 2 && (tall >> rs & 1);
+                const int sub = is_tall ? lane >> 4 : lane >> 3, u = is_tall ? lane & 15 : lane & 7;      // row of the instruction, piece of the row
+                const bool swap = u & 4;                       // lanes of a row start with different units: no bank conflicts
+                const int k0 = (u & 3) * 2 + (swap ? 1 : 0), k1 = (u & 3) * 2 + (swap ? 0 : 1);
+#pragma unroll
+                for (int b = 0; b < 8; b += 4) {
+                    uint4 x[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4 *>(src + 512 * (b + j));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        // row of the stage: tall 16 fw + 2 i + sub; else 64 (i / 4) + 16 fw + 4 (i % 4) + sub
+                        const int i = b + j, r = is_tall ? 16 * fw + 2 * i + sub : 64 * (i >> 2) + 16 * fw + 4 * (i & 3) + sub;
+                        uint4 a, c;
+                        widen4<T>(x[j].x, a.x, a.y);
+                        widen4<T>(x[j].y, a.z, a.w);
+                        widen4<T>(x[j].z, c.x, c.y);
+                        widen4<T>(x[j].w, c.z, c.w);
+                        unsigned char *const at = dst + (r >> 3) * (is_tall ? 4096 : 2048) + (u >> 2) * 1024 + (r & 7) * 128;
+                        *reinterpret_cast<uint4 *>(at + ((k0 ^ (r & 7)) << 4)) = swap ? c : a;
+                        *reinterpret_cast<uint4 *>(at + ((k1 ^ (r & 7)) << 4)) = swap ? a : c;
+                    }
+                }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(s32(&S.full[cc.idx]));
+                ++done;
+                cc.advance(1);
+            };
+            PageCursor pc[2];
+            long long off[2], noff[2] = {0, 0};
+            int rows[2], nrows[2] = {0, 0};
+            const auto locate = [&](long long (&o)[2], int (&n)[2]) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    int at;
+                    const int page = pc[g].take(at, n[g]);
+                    o[g] = page < 0 ? 0ll : page * P.page_stride + wk.hk * P.head_stride + at * P.tok_stride;
+                }
+            };
+            const auto issue = [&](bool is_tall) {
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                tall = (tall & ~(1u << issued % C::kRaw)) | (is_tall ? 1u : 0u) << issued % C::kRaw;
+                ++issued;
+                if (issued >= C::kRaw) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 1) : "memory");
+                    widen();
+                }
+            };
+            const long long two = 2 * P.tok_stride, four = 4 * P.tok_stride;
+            const auto fetch_wide = [&](const void *pool, const long long (&o)[2], const int (&n)[2], int dim) {
+                const uint32_t to = raw + (issued % C::kRaw) * kRawBytes;
+                const int sub = lane >> 3;
+                const unsigned char *const from = static_cast<const unsigned char *>(pool) + dim + 16 * (lane & 7) + sub * P.tok_stride;
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const unsigned char *src = from + o[g];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j, src += four) {
+                        const bool real = 4 * j + sub < n[g];
+                        copy16(to + 512 * (4 * g + j), real ? src : static_cast<const unsigned char *>(pool), real);
+                    }
+                }
+                issue(false);
+            };
+            const auto fetch_tall = [&](const void *pool, long long o, int n) {
+                const uint32_t to = raw + (issued % C::kRaw) * kRawBytes;
+                const int sub = lane >> 4;
+                const unsigned char *src = static_cast<const unsigned char *>(pool) + o + 16 * (lane & 15) + sub * P.tok_stride;
+#pragma unroll
+                for (int j = 0; j < 8; ++j, src += two) {
+                    const bool real = 2 * j + sub < n;
+                    copy16(to + 512 * j, real ? src : static_cast<const unsigned char *>(pool), real);
+                }
+                issue(true);
+            };
+            while (ok && wk.next()) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) pc[g].begin(P, wk.b, wk.blk * kTok + 64 * g + 16 * fw, wk.s.len);
+                locate(off, rows);
+                for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, off, rows, h * kDims);
+                for (int i = 0; i < wk.nb && ok; ++i) {
+                    if (i + 1 < wk.nb) {
+                        locate(noff, nrows);
+                        for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, noff, nrows, h * kDims);
+                    }
+                    if constexpr (H == 2) {
+                        for (int h = 0; h < 2 && ok; ++h) fetch_tall(P.v, off[h], rows[h]);
+                    } else if (ok) {
+                        fetch_wide(P.v, off, rows, 0);
+                    }
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) { off[g] = noff[g]; rows[g] = nrows[g]; }
+                }
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            while (ok && done < issued) widen();
         }
     }
     fence_before_sync();
@@ -686,19 +868,21 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant
     }
 }
 
-// Joins the partial results: CTA (c, y) takes the pair whose blocks begin in CTA c's piece and end behind it, eight rows of
-// its tile, one warp per row.
+// Joins the partial results: CTA (c, y) takes the pair whose blocks begin in CTA c's piece and end behind it, 32 rows x 64
+// dimensions of its tile; lane = row, a warp has eight dimensions; the result turns in shared memory.
+constexpr int kMergeCols = 64;
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Params P) {
-    constexpr int kVec = HD / 128;                             // float4 per lane
+    __shared__ T turn[32][kMergeCols + 8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
-    const int lane = threadIdx.x & 31, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row0 = blockIdx.y / (HD / kMergeCols) * 32, col0 = blockIdx.y % (HD / kMergeCols) * kMergeCols;
     int m = 0, cta0 = 0;
     while (m < P.tiles && (int)blockIdx.x >= cta0 + P.plan[m]) cta0 += P.plan[m++];
     if (m >= P.tiles) return;
     const int W = P.plan[m], U = P.plan[kMaxTiles + m], w = blockIdx.x - cta0;
-    const int u0 = cut(U, W, w), u1 = cut(U, W, w + 1);
+    const int u0 = piece(U, W, w), u1 = piece(U, W, w + 1);
     if (u1 <= u0 || w + 1 >= W) return;
     const int *const prefix = P.plan + 2 * kMaxTiles + (size_t)m * (P.batch + 1);
     int lo = 0, hi = P.batch - 1;
@@ -711,103 +895,51 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     const int hk = (u1 - 1 - base) / nblk, begin = base + hk * nblk, end = begin + nblk;
     if (begin < u0 || end <= u1) return;
     const Seq s = seq_of(P, b);
-    if (row >= min(kM, s.rows - kM * m)) return;
-    int last = w + 1;                                          // the CTAs w .. last hold parts of it
-    while (last + 1 < W && cut(U, W, last + 1) < end) ++last;
-    const auto slot = [&](int k) { return (size_t)(2 * (cta0 + k) + (k == w && begin != u0 ? 1 : 0)) * P.rows_ws + row; };
+    const int rows = min(kM, s.rows - kM * m) - row0;          // of these 32
+    if (rows <= 0) return;
+    int parts = 2;                                             // the CTAs w .. w + parts - 1 hold blocks of it
+    while (w + parts < W && piece(U, W, w + parts) < end) ++parts;
+    const int first = 2 * (cta0 + w) + (begin != u0 ? 1 : 0), next = 2 * (cta0 + w + 1);     // slots: first, next, next + 2, ..
+    const int row = row0 + min(lane, rows - 1);
+    const auto slot = [&](int k) { return (size_t)(k ? next + 2 * (k - 1) : first); };
     float top = -INFINITY;
-    for (int k = w + lane; k <= last; k += 32)
-        if (cut(U, W, k) < cut(U, W, k + 1)) top = fmaxf(top, __ldcg(P.part_ml + 2 * slot(k)));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float4 acc[kVec];
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-    for (int k0 = w; k0 <= last; k0 += 32) {
-        float wt = 0.f, l = 0.f;
-        bool has = false;
-        if (k0 + lane <= last && cut(U, W, k0 + lane) < cut(U, W, k0 + lane + 1)) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(P.part_ml + 2 * slot(k0 + lane)));
-            has = ml.x != -INFINITY || ml.y != 0.f;            // parts in which the row saw nothing are zeros (a NaN is not)
-            wt = has ? exp2f(ml.x - top) : 0.f;
-            l = has ? ml.y * wt : 0.f;
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        sum += l;
-        const uint32_t any = __ballot_sync(0xffffffffu, has);
-        const int count = min(32, last - k0 + 1);
 #pragma unroll 4
-        for (int j = 0; j < count; ++j) {
-            const float f = __shfl_sync(0xffffffffu, wt, j);
-            if (!(any >> j & 1)) continue;
-            const float4 *const src = reinterpret_cast<const float4 *>(P.part_o + slot(k0 + j) * HD) + lane;
+    for (int k = 0; k < parts; ++k) top = fmaxf(top, __ldcg(P.part_ml + 2 * slot(k) * P.rows_ws + row));
+    float acc[8] = {}, sum = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < parts; ++k) {
+        const float *const ml = P.part_ml + 2 * slot(k) * P.rows_ws + row;
+        const float mk = __ldcg(ml), lk = __ldcg(ml + P.rows_ws);
+        const float4 *const src = reinterpret_cast<const float4 *>(P.part_o) + (slot(k) * (HD / 4) + col0 / 4 + 2 * warp) * P.rows_ws + row;
+        const float4 v0 = __ldcg(src), v1 = __ldcg(src + P.rows_ws);
+        const float v[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+        if (mk != -INFINITY || lk != 0.f) {                    // parts in which the row saw nothing are zeros (a NaN is not)
+            const float f = exp2f(mk - top);
+            sum += lk * f;
 #pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const float4 x = __ldcg(src + 32 * v);
-                acc[v].x += x.x * f; acc[v].y += x.y * f; acc[v].z += x.z * f; acc[v].w += x.w * f;
-            }
+            for (int e = 0; e < 8; ++e) acc[e] += v[e] * f;
         }
     }
     const float inv = sum == 0.f ? 0.f : P.v_scale / sum;
-    const int R = kM * m + row, i = R / P.G;
-    T *const out = static_cast<T *>(P.out) + (size_t)(s.first + i) * P.out_stride + (size_t)(hk * P.G + R - i * P.G) * HD;
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-        uint2 r;
-        r.x = Type16<T>::pack(acc[v].x * inv, acc[v].y * inv);
-        r.y = Type16<T>::pack(acc[v].z * inv, acc[v].w * inv);
-        *reinterpret_cast<uint2 *>(out + 128 * v + 4 * lane) = r;
+    for (int e = 0; e < 8; e += 2)
+        *reinterpret_cast<uint32_t *>(&turn[lane][8 * warp + e]) = Type16<T>::pack(acc[e] * inv, acc[e + 1] * inv);
+    __syncthreads();
+    const int r = threadIdx.x >> 3, x = threadIdx.x & 7;       // eight lanes write the 128 bytes of a row
+    if (r < rows) {
+        const int R = kM * m + row0 + r, i = R / P.G;
+        T *const out = static_cast<T *>(P.out) + (size_t)(s.first + i) * P.out_stride + (size_t)(hk * P.G + R - i * P.G) * HD + col0;
+        *reinterpret_cast<uint4 *>(out + 8 * x) = *reinterpret_cast<const uint4 *>(&turn[r][8 * x]);
     }
 }
 
 // ---------------------------------------------------------------- host side
-using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        else
-            cudaGetLastError();
-    }
-    return fn;
-}
-
-// 16-bit pools: (64 values, token, 64-value chunk, head, page), boxes of 8 tokens x 2 chunks, 128-byte swizzle: a box is two
-// 1 KB swizzle atoms.  e4m3 pools: (byte, token, head, page), boxes of 16 tokens x 128 bytes, as they lie.
-static bool make_map(CUtensorMap *map, void *pool, const exl3_paged_cache &c) {
-    const EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    const bool fp8 = c.dtype == EXL3_KV_E4M3;
-    const cuuint64_t e = fp8 ? 1 : 2;
-    const cuuint64_t hd = c.head_dim, page = c.page_size, heads = c.kv_heads, pages = c.num_pages;
-    const cuuint64_t ts = c.token_stride * e, hs = c.head_stride * e, ps = c.page_stride * e;
-    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
-    if (fp8) {
-        const cuuint64_t dims[4] = {hd, page, heads, pages}, strides[3] = {ts, hs, ps};
-        const cuuint32_t box[4] = {kDims, 16, 1, 1};
-        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    }
-    const cuuint64_t dims[5] = {64, page, hd / 64, heads, pages}, strides[4] = {ts, 128, hs, ps};
-    const cuuint32_t box[5] = {64, 8, 2, 1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, pool, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 struct Sizes { int tiles, rows_ws; size_t plan, ml, total; };
 static Sizes sizes_of(int batch, int G, int max_drafts, int hd) {
     Sizes z;
     const int rows = max_drafts * G;
     z.tiles = (rows + kM - 1) / kM;
-    z.rows_ws = rows < kM ? rows : kM;
+    z.rows_ws = rows < kM ? (rows + 31) / 32 * 32 : kM;
     z.plan = ((size_t)(2 * kMaxTiles + (size_t)z.tiles * (batch + 1)) * 4 + 255) & ~(size_t)255;
     z.ml = ((size_t)2 * kMaxGrid * z.rows_ws * 8 + 255) & ~(size_t)255;
     z.total = z.plan + z.ml + (size_t)2 * kMaxGrid * z.rows_ws * hd * 4;
@@ -815,7 +947,7 @@ static Sizes sizes_of(int batch, int G, int max_drafts, int hd) {
 }
 
 template <typename T, bool FP8, int HD>
-static int launch(const CUtensorMap &kmap, const CUtensorMap &vmap, const Params &P, cudaStream_t st) {
+static int launch(const Params &P, cudaStream_t st) {
     using C = Cfg<FP8, HD>;
     auto kernel = tree_attn_kernel<T, FP8, HD>;
     static bool ready[64] = {};
@@ -828,8 +960,8 @@ static int launch(const CUtensorMap &kmap, const CUtensorMap &vmap, const Params
         }
         if (dev >= 0 && dev < 64) ready[dev] = true;
     }
-    if (launch_pdl(kernel, dim3(kMaxGrid), dim3(C::kThreads), C::kSmem, st, kmap, vmap, P) != cudaSuccess) return EXL3_E_LAUNCH;
-    if (launch_pdl(tree_merge_kernel<T, HD>, dim3(kMaxGrid, (P.rows_ws + 7) / 8), dim3(256), 0, st, P) != cudaSuccess)
+    if (launch_pdl(kernel, dim3(kMaxGrid), dim3(C::kThreads), C::kSmem, st, P) != cudaSuccess) return EXL3_E_LAUNCH;
+    if (launch_pdl(tree_merge_kernel<T, HD>, dim3(kMaxGrid, P.rows_ws / 32 * (HD / kMergeCols)), dim3(256), 0, st, P) != cudaSuccess)
         return EXL3_E_LAUNCH;
     return launch_status();
 }
@@ -881,7 +1013,7 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     if (!aligned(workspace, 16)) return EXL3_E_ALIGN;
     Params P = {};
     P.q = q; P.out = out; P.q_stride = q_stride; P.out_stride = out_stride;
-    P.v = cache->v_pages;
+    P.k = cache->k_pages; P.v = cache->v_pages;
     P.page_stride = cache->page_stride; P.head_stride = cache->head_stride; P.tok_stride = cache->token_stride;
     P.block_table = (const int *)block_table; P.seq_lens = (const int *)seq_lens; P.starts = (const int *)starts;
     P.mask = (const long long *)mask;
@@ -895,16 +1027,14 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     P.plan = (int *)workspace;
     P.part_ml = (float *)((char *)workspace + z.plan);
     P.part_o = (float *)((char *)workspace + z.plan + z.ml);
-    CUtensorMap kmap, vmap;
-    if (!make_map(&kmap, cache->k_pages, *cache) || !make_map(&vmap, cache->v_pages, *cache)) return EXL3_E_LAUNCH;
     const bool fp8 = cache->dtype == EXL3_KV_E4M3;
     cudaStream_t st = (cudaStream_t)stream;
     if (hd == 256) {
-        if (is_bf16) return fp8 ? launch<__nv_bfloat16, true, 256>(kmap, vmap, P, st) : launch<__nv_bfloat16, false, 256>(kmap, vmap, P, st);
-        return fp8 ? launch<__half, true, 256>(kmap, vmap, P, st) : launch<__half, false, 256>(kmap, vmap, P, st);
+        if (is_bf16) return fp8 ? launch<__nv_bfloat16, true, 256>(P, st) : launch<__nv_bfloat16, false, 256>(P, st);
+        return fp8 ? launch<__half, true, 256>(P, st) : launch<__half, false, 256>(P, st);
     }
-    if (is_bf16) return fp8 ? launch<__nv_bfloat16, true, 128>(kmap, vmap, P, st) : launch<__nv_bfloat16, false, 128>(kmap, vmap, P, st);
-    return fp8 ? launch<__half, true, 128>(kmap, vmap, P, st) : launch<__half, false, 128>(kmap, vmap, P, st);
+    if (is_bf16) return fp8 ? launch<__nv_bfloat16, true, 128>(P, st) : launch<__nv_bfloat16, false, 128>(P, st);
+    return fp8 ? launch<__half, true, 128>(P, st) : launch<__half, false, 128>(P, st);
 }
 
 extern "C" int exl3_tree_attn_status(unsigned *status_out) {
