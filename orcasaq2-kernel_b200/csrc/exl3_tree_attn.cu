@@ -5,16 +5,18 @@
 //     S[row][token] = Q (shared memory) x K^T (shared memory, K-major)          fp32 in tensor memory
 //     P = exp2(S * scale - m), rounded to 16 bits, in place of S                tensor memory
 //     O[row][dim]  += P (tensor memory) x V (shared memory, MN-major: V lies [token][dim] as the cache has it)
-// Two threads share a row (a TMEM lane), 64 scores of the block each, held in registers: no shuffles, one exchange of
-// the maximum through shared memory.
+// Two groups of four warps take the blocks in turn, thread = row = TMEM lane: no shuffles, and while one group is at its
+// exponentials the other waits, loads or stores (eight warps on one block at a time: 2.8 to 3.2 thousand cycles a block,
+// all latencies in a row).  A row's maximum goes from group to group through shared memory.
 //
 // What bounds it: K and V are read once per 128 rows, 4 * HD * 128 * 128 multiply-adds for 4 * HD * 128 bytes; at 128
 // rows the tensor cores need a third of the time that HBM takes, so up to 128 rows the kernel's business is to keep
-// loads in flight: a ring of 32 KB stages (128 tokens x 128 dimensions of K, 64 x 256 or 128 x 128 of V), filled by four
-// warps with 16-byte cp.async straight into the swizzled places, each thread's arrival on the stage's barrier following
-// its copies.  (TMA boxes were measured first: pages allow boxes of 8 or 16 tokens only, and sixteen 2 KB boxes took
-// 1700 cycles a stage, whether the bytes came from HBM or from L2.)  More rows are more tiles: CTAs of the tiles of one
-// sequence walk the same blocks at the same time and share them in L2.
+// loads in flight: a ring of 32 KB stages (128 tokens x 128 dimensions of K, 64 x 256 or 128 x 128 of V), each filled by
+// a warp of its own with 16-byte cp.async straight into the swizzled places; each lane's arrival on the stage's barrier
+// follows its copies.  (TMA boxes were measured first: pages allow boxes of 8 or 16 tokens only, and
+// issuing sixteen 2 KB boxes a stage bounds the rate at 7.2 TB/s over the GPU even out of L2, where cp.async reaches 18.
+// With four warps on every stage each of them paid four waits a block.)  More rows are more tiles: CTAs of the tiles
+// of one sequence walk the same blocks at the same time and share them in L2.
 // Work is split evenly whatever the lengths: the blocks of all (sequence, KV head) pairs form one line, every CTA
 // takes an equal piece of it (found from the lengths on the device), and a pair that several CTAs share leaves partial
 // sums with their maximum, which a second kernel joins in order (fixed order: the same bytes every run).
@@ -25,9 +27,9 @@
 // filled with zeros instead of read, and non-finite V values of drafts, which some rows see and others do not, are
 // zeroed before the product and added to the rows that see them at the end (a path that finite caches never take).
 //
-// e4m3 caches: the four warps fetch 16 KB raw stages, every thread its own pieces (so it waits for nobody else's), and
-// widen them exactly to the 16-bit type of q into the swizzled stages; the scales fold into the softmax scale and the
-// normalisation.
+// e4m3 caches: a pair of warps per stage fetches a raw stage of 16 KB beside it, every thread its own pieces (so it waits for nobody
+// else's), and widen them exactly to the 16-bit type of q into the swizzled stages, refilling the raw stage piece by
+// piece as they go; the scales fold into the softmax scale and the normalisation.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -73,13 +75,15 @@ struct Params {
 };
 
 struct Shared {
-    uint64_t full[6], empty[6];
-    uint64_t s_full[2], p_ready[2], v_here[2], pv_done[2], q_full, q_empty, o_free, drain;
+    // A stage has a barrier for K and one for V: each of the two threads that issue MMAs sees only the rounds that are
+    // its own (with one barrier a thread could be a whole round behind another's, and parity would mislead it).
+    uint64_t k_full[5], v_full[5], empty[5];
+    uint64_t s_full[2], p_ready[2], v_here[2], pv_done[2], q_full, q_empty, o_free, drain[2];
     uint32_t tmem_base;
     int nonfinite[2];                         // of the current segment and the one before, in turn
-    float top[2][2][kM];                      // maxima of the two halves of a row, two blocks
+    float top[kM], sum[2][kM];                // of the rows; sums of the two groups
     int total[kMaxTiles];
-    int sums[16];                             // one per warp
+    int sums[20];                             // one per warp
     int first_seq, first_off;
 };
 static_assert(sizeof(Shared) <= 3072, "shared state");
@@ -88,9 +92,9 @@ template <bool FP8, int HD>
 struct Cfg {
     static constexpr int kHalves = HD / kDims;                       // stages of a K or V block
     static constexpr int kQBytes = kM * HD * 2;
-    static constexpr int kStages = FP8 ? 3 : (HD == 256 ? 5 : 6);
-    static constexpr int kRaw = FP8 ? 4 : 0;
-    static constexpr int kThreads = 512;          // 1 MMA + 3 query + 8 softmax + 4 fetch warps
+    static constexpr int kStages = FP8 ? 3 : 5;
+    static constexpr int kRaw = FP8 ? kStages : 0;
+    static constexpr int kThreads = 32 * (11 + (FP8 ? 2 : 1) * kStages);     // 2 MMA + 1 query + 8 softmax warps, one or two per stage
     static constexpr int kSmem = kQBytes + kStages * kStageBytes + kRaw * kRawBytes + sizeof(Shared);
 };
 
@@ -98,6 +102,9 @@ struct Cfg {
 // Sixteen bytes into shared memory, or zeros.
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src) {      // (without a size: a fifth quicker out of L2)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 // This thread's arrival on the barrier once its copies so far have landed.
 __device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
@@ -136,15 +143,23 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&v)[32
           "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]),
           "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
+          "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]) : "memory");
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// The two warps of a quarter of the rows; all eight softmax warps.
-__device__ __forceinline__ void pair_sync(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory"); }
-__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 5, 256;" ::: "memory"); }
+// From a warp of one group to the warp of the same rows in the other (each id has one arriving and one waiting warp);
+// all eight softmax warps.
+__device__ __forceinline__ void pass_on(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void take_over(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 9, 256;" ::: "memory"); }
 // Two fp32 operations at a time.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -224,28 +239,23 @@ __device__ __forceinline__ int piece(int U, int W, int w) {
     return w * q + min(w, U - q * W);
 }
 
-// The pages of the sixteen-token (or shorter) pieces at t, t + 128, t + 256 .. of a sequence, one lookup ahead.
-struct PageCursor {
-    const int *row;                    // of the block table
-    int t, len, idx, at, size, step_idx, step_at, num_pages, ahead;
-    __device__ __forceinline__ void begin(const Params &P, int b, int tok, int length) {
-        row = P.block_table + (size_t)b * P.bt_stride;
-        t = tok; len = length; size = P.page_size; num_pages = P.num_pages;
-        idx = t / size; at = t - idx * size;
-        step_idx = kTok / size; step_at = kTok - step_idx * size;
-        ahead = t < len ? __ldg(row + idx) : -1;
-    }
-    // (page, token in the page) of the current piece, page -1 when none of it is there; then on to the next
-    __device__ __forceinline__ int take(int &in_page, int &tokens) {
-        const int page = (unsigned)ahead < (unsigned)num_pages ? ahead : -1;
-        in_page = at;
-        tokens = page < 0 ? 0 : len - t;
-        t += kTok; idx += step_idx; at += step_at;
-        if (at >= size) { at -= size; ++idx; }
-        ahead = t < len ? __ldg(row + idx) : -1;
-        return page;
-    }
-};
+// The page of the sixteen tokens at t of sequence b, -1 when they are on none.
+__device__ __forceinline__ int page_of(const Params &P, int b, int t, int len, int &at) {
+    const int idx = t / P.page_size;
+    at = t - idx * P.page_size;
+    return t < len ? __ldg(P.block_table + (size_t)b * P.bt_stride + idx) : -1;
+}
+
+// The stages of a segment in the order of the ring: K(0), then K(i + 1) (if there is one) and V(i) for every block i, H
+// stages each.  Stage j of the segment:
+struct Fill { int block, half; bool is_v; };
+template <int H>
+__device__ __forceinline__ Fill fill_of(int j, int nb) {
+    if (j < H) return Fill{0, j, false};
+    const int q = (j - H) / (2 * H), r = (j - H) % (2 * H);
+    if (q < nb - 1 && r < H) return Fill{q + 1, r, false};
+    return Fill{q, r % H, true};
+}
 
 // ---------------------------------------------------------------- e4m3 -> 16 bits
 template <typename T>
@@ -283,10 +293,10 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     }
 
     if (tid == 0) {
-        for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.full[i]), FP8 ? 4 : 128); mbar_init(s32(&S.empty[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 8); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
-        mbar_init(s32(&S.q_full), 96); mbar_init(s32(&S.q_empty), 1);
-        mbar_init(s32(&S.o_free), 8); mbar_init(s32(&S.drain), 1);
+        for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.k_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.v_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.empty[i]), 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 4); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
+        mbar_init(s32(&S.q_full), 32); mbar_init(s32(&S.q_empty), 1);
+        mbar_init(s32(&S.o_free), 8); mbar_init(s32(&S.drain[0]), 1); mbar_init(s32(&S.drain[1]), 1);
         S.nonfinite[0] = S.nonfinite[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
@@ -359,65 +369,88 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     if (u1 > u0) {
         Walk wk(P, m, S.first_seq, S.first_off, u1 - u0);
         if (warp == 1) {
-            // ---------------- the MMAs
+            // ---------------- S = Q K^T.  Two threads issue the MMAs, one for each product: a thread's waits, fences and
+            // commits cost it about as much as the tensor cores need for its share of a block (one thread for both: 5050
+            // cycles a block, of which the tensor cores worked 2300)
             if (lane == 0) {
                 constexpr uint32_t kType = __is_same(T, __half) ? 0u : (1u << 7 | 1u << 10);
-                const uint32_t id_qk = umma_idesc_f16(kM, kTok) | kType | (P.negate ? 1u << 13 : 0u);      // bit 13: -A
-                const uint32_t id_pv = umma_idesc_f16(kM, HD) | kType | 1u << 16;                          // bit 16: B is MN-major
-                Cursor rc(0, C::kStages);
+                const uint32_t idesc = umma_idesc_f16(kM, kTok) | kType | (P.negate ? 1u << 13 : 0u);      // bit 13: -A
+                const uint64_t qdesc = desc_sw128(s32(smQ), 16, 1024), kdesc = desc_sw128(s32(ring), 16, 2048);
+                uint32_t phases = 0;                           // of the stages' K barriers
+                int stage = 0, cnt = 0;
                 bool ok = true;
-                int cnt = 0;                                   // blocks whose probabilities were used
-                const auto scores = [&](int n) {               // S(n) = Q K^T
-                    const uint32_t d = tmem + HD + (n & 1) * kTok;
-                    for (int h = 0; h < H && ok; ++h, rc.advance(1)) {
-                        ok = mbar_wait(s32(&S.full[rc.idx]), rc.phase, status);
-                        if (!ok) return;
-                        if constexpr (!FP8) fence_async();     // the copies were the other warps', plain ones
-                        fence_after_sync();
-                        const uint32_t kb = s32(ring + (size_t)rc.idx * kStageBytes);
-#pragma unroll
-                        for (int k = 0; k < kDims / 16; ++k)
-                            umma_f16_ss(d, desc_sw128(s32(smQ) + (2 * h + k / 4) * (kM * 128) + (k % 4) * 32, 16, 1024),
-                                        desc_sw128(kb + (k / 4) * 1024 + (k % 4) * 32, 16, 2048), id_qk, h || k);
-                        umma_commit(s32(&S.empty[rc.idx]));
-                    }
-                    umma_commit(s32(&S.s_full[n & 1]));
-                };
                 while (ok && wk.next()) {
                     ok = mbar_wait(s32(&S.q_full), wk.index & 1, status);
                     if (!ok) break;
-                    fence_async();
-                    fence_after_sync();
-                    scores(cnt);
-                    if (wk.nb == 1) umma_commit(s32(&S.q_empty));
+                    fence_async();                             // the copies were other warps', plain ones
                     for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
-                        if (i + 1 < wk.nb) {
-                            scores(cnt + 1);
-                            if (i + 2 == wk.nb) umma_commit(s32(&S.q_empty));
+                        if (cnt >= 2) ok = mbar_wait(s32(&S.pv_done[cnt & 1]), ((cnt - 2) >> 1) & 1, status);   // P(cnt - 2) was used
+                        const uint32_t d = tmem + HD + (cnt & 1) * kTok;
+                        for (int h = 0; h < H && ok; ++h) {
+                            ok = mbar_wait(s32(&S.k_full[stage]), phases >> stage & 1, status);
+                            if (!ok) break;
+                            phases ^= 1u << stage;
+                            if constexpr (!FP8) fence_async();
+                            fence_after_sync();
+                            const uint64_t kd = kdesc + (uint32_t)(stage * (kStageBytes >> 4)), qd = qdesc + (uint32_t)(h * (2 * kM * 128 >> 4));
+#pragma unroll
+                            for (int k = 0; k < kDims / 16; ++k)
+                                umma_f16_ss(d, qd + ((k / 4) * (kM * 128) + (k % 4) * 32 >> 4), kd + ((k / 4) * 1024 + (k % 4) * 32 >> 4), idesc, h || k);
+                            umma_commit(s32(&S.empty[stage]));
+                            if (++stage == C::kStages) stage = 0;
                         }
-                        Cursor vc = rc;
-                        for (int h = 0; h < H && ok; ++h, vc.advance(1)) ok = mbar_wait(s32(&S.full[vc.idx]), vc.phase, status);
-                        if (ok) mbar_arrive(s32(&S.v_here[cnt & 1]));
-                        if (ok) ok = mbar_wait(s32(&S.p_ready[cnt & 1]), (cnt >> 1) & 1, status);
+                        umma_commit(s32(&S.s_full[cnt & 1]));
+                        // over V(i - 1) to the next K; behind the last K lie V of the last two blocks
+                        const int skip = i + 1 == wk.nb ? (wk.nb > 1 ? 2 * H : H) : i ? H : 0;
+                        stage = (stage + skip) % C::kStages;
+                    }
+                    umma_commit(s32(&S.q_empty));
+                }
+                umma_commit(s32(&S.drain[0]));
+                mbar_wait(s32(&S.drain[0]), 0, status);
+            }
+        } else if (warp == 0) {
+            // ---------------- O += P V
+            if (lane == 0) {
+                constexpr uint32_t kType = __is_same(T, __half) ? 0u : (1u << 7 | 1u << 10);
+                const uint32_t idesc = umma_idesc_f16(kM, HD) | kType | 1u << 16;                          // bit 16: B is MN-major
+                const uint64_t vdesc = desc_sw128(s32(ring), 1024, HD * 16);
+                uint32_t phases = 0;
+                int stage = 0, cnt = 0;
+                bool ok = true;
+                while (ok && wk.next()) {
+                    for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
+                        // before V(i) lies K(i + 1), before V(0) also K(0)
+                        stage = (stage + (i + 1 < wk.nb ? H : 0) + (i ? 0 : H)) % C::kStages;
+                        int st = stage;
+                        for (int h = 0; h < H && ok; ++h) {
+                            ok = mbar_wait(s32(&S.v_full[st]), phases >> st & 1, status);
+                            phases ^= 1u << st;
+                            if (++st == C::kStages) st = 0;
+                        }
+                        if (!ok) break;
+                        mbar_arrive(s32(&S.v_here[cnt & 1]));
+                        ok = mbar_wait(s32(&S.p_ready[cnt & 1]), (cnt >> 1) & 1, status);
                         if (ok && i == 0 && wk.index) ok = mbar_wait(s32(&S.o_free), (wk.index - 1) & 1, status);
                         if (!ok) break;
                         if constexpr (!FP8) fence_async();
                         fence_after_sync();
-                        for (int h = 0; h < H; ++h, rc.advance(1)) {
-                            const uint32_t vb = s32(ring + (size_t)rc.idx * kStageBytes);
-                            const uint32_t p = tmem + HD + (cnt & 1) * kTok + h * (kTok / H / 2);
+                        for (int h = 0; h < H; ++h) {
+                            const uint64_t vd = vdesc + (uint32_t)(stage * (kStageBytes >> 4));
+                            const uint32_t p = tmem + HD + (cnt & 1) * kTok + h * 32;
 #pragma unroll
                             for (int k = 0; k < kTok / H / 16; ++k)
-                                umma_f16_ts(tmem, p + 8 * k, desc_sw128(vb + k * (HD * 32), 1024, HD * 16), id_pv, i || h || k);
-                            umma_commit(s32(&S.empty[rc.idx]));
+                                umma_f16_ts(tmem, p + k * 8, vd + (k * (HD * 32) >> 4), idesc, i || h || k);
+                            umma_commit(s32(&S.empty[stage]));
+                            if (++stage == C::kStages) stage = 0;
                         }
                         umma_commit(s32(&S.pv_done[cnt & 1]));
                     }
                 }
-                umma_commit(s32(&S.drain));
-                mbar_wait(s32(&S.drain), 0, status);
+                umma_commit(s32(&S.drain[1]));
+                mbar_wait(s32(&S.drain[1]), 0, status);
             }
-        } else if (warp < 4) {
+        } else if (warp == 2) {
             // ---------------- query rows into shared memory (swizzled, K-major), rows behind the last one zero
             constexpr int kUnits = HD / 8, kRows = 32 / kUnits;   // 16-byte units of a row, rows of an instruction
             bool ok = true;
@@ -425,21 +458,22 @@ tree_attn_kernel(const __grid_constant__ Params P) {
             int filled = kM;                                   // rows that may hold something
             while (ok && wk.next()) {
                 if (wk.index) {
-                    ok = mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status);
+                    ok = mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status, 200);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                 }
                 const int rows = wk.rows(), upto = max(filled, rows);
-                constexpr int kStep = 3 * kRows;
-                int r = (warp ? warp - 1 : 0) * kRows + sub, i = (kM * m + r) / P.G, g = kM * m + r - i * P.G;
-                const T *const base = static_cast<const T *>(P.q) + (size_t)wk.s.first * P.q_stride + (size_t)wk.hk * P.G * HD + 8 * u;
-                const uint32_t dst = s32(smQ) + (u >> 3) * (kM * 128);
+                constexpr int kStep = kRows;
+                int r = sub, i = (kM * m + r) / P.G, g = kM * m + r - i * P.G;
+                const T *src = static_cast<const T *>(P.q) + (size_t)(wk.s.first + i) * P.q_stride + (size_t)(wk.hk * P.G + g) * HD + 8 * u;
                 const int di = kStep / P.G, dg = kStep - di * P.G;
+                const long long step = di * P.q_stride + dg * HD, wrap = P.q_stride - (long long)P.G * HD;
+                const uint32_t dst = s32(smQ) + (u >> 3) * (kM * 128);
 #pragma unroll 4
                 for (; r < rows; r += kStep) {
-                    copy16(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4), base + i * P.q_stride + g * HD, true);
-                    i += di; g += dg;
-                    if (g >= P.G) { g -= P.G; ++i; }
+                    copy16(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4), src);
+                    src += step; g += dg;
+                    if (g >= P.G) { g -= P.G; src += wrap; }
                 }
                 for (; r < upto; r += kStep)
                     *reinterpret_cast<uint4 *>(smQ + (u >> 3) * (kM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
@@ -448,11 +482,11 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 arrive_behind_copies(s32(&S.q_full));
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-        } else if (warp < 12) {
-            // ---------------- softmax: a thread has 64 scores of its row (TMEM lane)
-            const int quarter = warp & 3, row = 32 * quarter + lane, side = (warp - 4) >> 2;
+        } else if (warp < 11) {
+            // ---------------- softmax: thread = row = TMEM lane; group `side` takes the blocks of its parity
+            const int quarter = warp & 3, row = 32 * quarter + lane, side = (warp - 3) >> 2;
             const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
-            constexpr int kCols = HD / 2;                      // of O, this thread's half
+            constexpr int kCols = HD / 2;                      // of the result, this thread's half
             const uint32_t o_t = tmem + lane_base + side * kCols;
             // These warps meet at barriers: after a wait that ran out they walk on without waiting (what they write is
             // garbage then, the status word says so).
@@ -470,96 +504,95 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 unsigned long long bits = 0;
                 if (live) bits = P.mask ? (unsigned long long)__ldg(P.mask + wk.s.first + draft) : (draft >= 63 ? ~0ull : (2ull << draft) - 1);
                 float top = -INFINITY;
-                float2 sum2 = make_float2(0.f, 0.f);           // of this thread's columns
-                PageCursor pc;                                 // lanes 0..3: sixteen tokens of this half each
-                pc.begin(P, wk.b, wk.blk * kTok + 64 * side + 16 * (lane & 3), wk.s.len);
-                for (int i = 0; i < wk.nb; ++i, ++cnt) {
-                    const int tok0 = (wk.blk + i) * kTok;
-                    int in_page, there;
-                    pc.take(in_page, there);
-                    const uint32_t groups = __ballot_sync(0xffffffffu, there > 0) & 0xFu;
-                    const bool masked = tok0 + kTok > ctx || groups != 0xFu;           // uniform in the warp
-                    uint32_t vis[2] = {~0u, ~0u};
-                    if (masked) {
+                float2 sum2 = make_float2(0.f, 0.f);           // over this group's blocks, relative to `top`
+                for (int i = (cnt ^ side) & 1; i < wk.nb; i += 2) {
+                    const int n = cnt + i, tok0 = (wk.blk + i) * kTok;         // n: number of the block in the CTA
+                    int at;
+                    const int t8 = tok0 + 16 * (lane & 7), page = page_of(P, wk.b, t8, wk.s.len, at);
+                    const uint32_t groups = __ballot_sync(0xffffffffu, t8 >= wk.s.len || (unsigned)page < (unsigned)P.num_pages) & 0xFFu;
+                    const bool masked = tok0 + kTok > ctx || groups != 0xFFu;          // uniform in the warp
+                    // which of the 32 tokens from tok0 + 32 k the row sees: context, then the drafts' bits shifted to their places
+                    const auto seen = [&](int k) {
+                        const int c = ctx - tok0 - 32 * k, l = wk.s.len - tok0 - 32 * k;
+                        uint32_t v = 0;
+                        if (c >= 32) v = ~0u;
+                        else if (c > 0) v = (1u << c) - 1 | (uint32_t)(bits << c);
+                        else v = -c < 64 ? (uint32_t)(bits >> -c) : 0u;
+                        if (l < 32) v &= l > 0 ? (1u << l) - 1 : 0u;
+                        v &= (groups >> (2 * k) & 1 ? 0xFFFFu : 0u) | (groups >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
+                        return live ? v : 0u;
+                    };
+                    // (The loops over four times 32 scores stay loops: unrolled, the code of the roles did not fit the instruction
+                    // caches, and the warps waited for instructions more often than for anything else but loads.)
+                    const auto load = [&](int k, uint32_t (&y)[32]) {          // scores, minus infinity where nothing is seen
+                        tmem_ld32(tmem + lane_base + HD + (n & 1) * kTok + 32 * k, y);
+                        const uint32_t vis = masked ? seen(k) : ~0u;
+                        tmem_wait_ld();
+                        if (masked) {
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int a = tok0 + 64 * side + 32 * k;
-                            uint32_t v = 0;
-                            // context tokens of these 32, then the drafts' bits shifted to their places
-                            const int c = ctx - a, l = wk.s.len - a;
-                            if (c >= 32) v = ~0u;
-                            else if (c > 0) v = (1u << c) - 1 | (uint32_t)(bits << c);
-                            else v = -c < 64 ? (uint32_t)(bits >> -c) : 0u;
-                            if (l < 32) v &= l > 0 ? (1u << l) - 1 : 0u;
-                            v &= (groups >> (2 * k) & 1 ? 0xFFFFu : 0u) | (groups >> (2 * k) & 2 ? 0xFFFF0000u : 0u);
-                            vis[k] = live ? v : 0u;
+                            for (int e = 0; e < 32; ++e) y[e] = vis >> e & 1 ? y[e] : 0xFF800000u;
                         }
-                    }
-                    const uint32_t s_t = tmem + lane_base + HD + (cnt & 1) * kTok;
-                    hold(&S.s_full[cnt & 1], (cnt >> 1) & 1);
-                    uint32_t x[2][32];
-                    tmem_ld32(s_t + 64 * side, x[0]);
-                    tmem_ld32(s_t + 64 * side + 32, x[1]);
-                    tmem_wait_ld();
+                    };
+                    const uint32_t s_t = tmem + lane_base + HD + (n & 1) * kTok;
+                    hold(&S.s_full[n & 1], (n >> 1) & 1);
                     float mx = -INFINITY;
-                    if (masked) {
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t y[32];
+                        load(k, y);
+                        float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int e = 0; e < 64; ++e) mx = fmaxf(mx, vis[e >> 5] >> (e & 31) & 1 ? __uint_as_float(x[e >> 5][e & 31]) : -INFINITY);
-                    } else {
-                        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                        for (int e = 0; e < 64; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(x[e >> 5][e & 31]));
+                        for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(y[e]));
                         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     }
-                    S.top[cnt & 1][side][row] = mx;
-                    fence_before_sync();
-                    pair_sync(quarter);                        // (after which both halves' scores are in registers, too)
-                    fence_after_sync();
-                    mx = fmaxf(mx, S.top[cnt & 1][side ^ 1][row]);
                     mx = mx == -INFINITY ? mx : mx * P.scale_log2;
+                    if (i > 0) {                               // the maximum as the block before left it
+                        take_over(1 + 4 * (side ^ 1) + quarter);
+                        const float before = top;
+                        top = S.top[row];
+                        if (top != before) { const float c = ex2(before - top); sum2.x *= c; sum2.y *= c; }
+                    }
                     const bool raise = mx > top + kRaise || (top == -INFINITY && mx > top);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float corr = raise ? ex2(top - mx) : 1.f;      // 0 when nothing was seen before
-                        if (raise) { top = mx; sum2.x *= corr; sum2.y *= corr; }
-                        if (i > 0) {
-                            hold(&S.pv_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1);
+                    const float corr = raise ? ex2(top - mx) : 1.f;    // 0 when nothing was seen before
+                    if (raise) { top = mx; sum2.x *= corr; sum2.y *= corr; }
+                    S.top[row] = top;
+                    if (__any_sync(0xffffffffu, raise) && i > 0) {
+                        hold(&S.pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
 #pragma unroll 1
-                            for (int c = 0; c < kCols; c += 32) {
-                                uint32_t o[32];
-                                tmem_ld32(o_t + c, o);
-                                tmem_wait_ld();
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(tmem + lane_base + c, o);
+                            tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st32(o_t + c, o);
-                            }
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                            tmem_st32(tmem + lane_base + c, o);
                         }
                     }
+                    if (i + 1 < wk.nb) pass_on(1 + 4 * side + quarter);
                     const float shift = top == -INFINITY ? 0.f : top;
                     const float2 mul = make_float2(P.scale_log2, P.scale_log2), sub = make_float2(-shift, -shift);
-                    uint32_t p[32];
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t y[32], p[16];
+                        load(k, y);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int k = e >> 4, c = 2 * (e & 15);
-                        float2 a = fma2(make_float2(__uint_as_float(x[k][c]), __uint_as_float(x[k][c + 1])), mul, sub);
-                        a.x = ex2(a.x);
-                        a.y = ex2(a.y);
-                        if (masked) {
-                            if (!(vis[k] >> c & 1)) a.x = 0.f;
-                            if (!(vis[k] >> (c + 1) & 1)) a.y = 0.f;
+                        for (int e = 0; e < 16; ++e) {
+                            float2 a = fma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), mul, sub);
+                            a.x = ex2(a.x);
+                            a.y = ex2(a.y);
+                            sum2 = add2(sum2, a);
+                            p[e] = Type16<T>::pack(a.x, a.y);
                         }
-                        sum2 = add2(sum2, a);
-                        p[e] = Type16<T>::pack(a.x, a.y);
+                        tmem_st16(s_t + 16 * k, p);            // over scores that were read
                     }
-                    tmem_st32(s_t + 32 * side, p);             // over scores that both threads have read
                     if (tok0 + kTok > ctx) {
                         // non-finite values of drafts become zeros (see the top of the file)
                         const int from = max(0, ctx - tok0), upto = min(kTok, wk.s.len - tok0);
                         const int vpos = pos + H + 2 * H * i + (i + 1 < wk.nb ? H : 0);
-                        // (announced by the MMA thread, which looks at every stage in its turn: the stage's own barrier may
-                        // still be a whole round behind, or ahead, of what this thread would wait for)
-                        hold(&S.v_here[cnt & 1], (cnt >> 1) & 1);
+                        // (announced by the MMA thread, which looks at every stage in its turn)
+                        hold(&S.v_here[n & 1], (n >> 1) & 1);
                         constexpr int kUnits = HD / 8, kRowsV = kTok / H;           // 16-byte units of a row, rows of a stage
-                        for (int e = tid - 128; e < (upto - from) * kUnits; e += 256) {
+                        for (int e = row; e < (upto - from) * kUnits; e += 128) {
                             const int r = from + e / kUnits, u = e % kUnits, st = (vpos + r / kRowsV) % C::kStages, q = r % kRowsV;
                             uint4 *const at = reinterpret_cast<uint4 *>(ring + (size_t)st * kStageBytes + (q >> 3) * (HD * 16) + (u >> 3) * 1024 +
                                                                         (q & 7) * 128 + (((u & 7) ^ (q & 7)) << 4));
@@ -574,16 +607,23 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     tmem_wait_st();
                     fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(s32(&S.p_ready[cnt & 1]));
+                    if (lane == 0) mbar_arrive(s32(&S.p_ready[n & 1]));
                 }
                 // ---- the segment's result
-                float sum = sum2.x + sum2.y;
-                S.top[cnt & 1][side][row] = sum;               // (the buffer of the block before last: read by all)
+                cnt += wk.nb;
+                softmax_sync();                                // S.top is the last block's now; and (for the group that had not the
+                                                               // last block) its scores have been there, so all products but two
                 hold(&S.pv_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1);
+                {
+                    const float before = top;
+                    top = S.top[row];
+                    const float c = top != before ? ex2(before - top) : 1.f;
+                    S.sum[side][row] = (sum2.x + sum2.y) * c;  // (0 * 0 when this group saw nothing)
+                }
                 softmax_sync();
-                sum = S.top[cnt & 1][0][row] + S.top[cnt & 1][1][row];
+                const float sum = S.sum[0][row] + S.sum[1][row];
                 const bool mend = S.nonfinite[wk.index & 1] != 0;       // uniform: all have written it before the barrier
-                if (tid == 128) S.nonfinite[wk.index & 1 ^ 1] = 0;      // read before the last barrier, written behind the next
+                if (tid == 96) S.nonfinite[wk.index & 1 ^ 1] = 0;      // read before the last barrier, written behind the next
                 const bool whole = wk.whole();
                 const float inv = sum == 0.f ? 0.f : P.v_scale / sum;
                 const int slot = 2 * blockIdx.x + (wk.index ? 1 : 0);
@@ -661,203 +701,184 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 pos += 2 * H * wk.nb;
             }
         } else if constexpr (!FP8) {
-            // ---------------- cache rows into the ring: a warp takes sixteen tokens of either half of a block
-            const int fw = warp - 12;
-            Cursor rc(0, C::kStages);
+            // ---------------- cache rows into the ring: warp f fills stage f (one warp waits for all of a stage's releases: with
+            // stages passed round it could be a whole round ahead of the others, and parity would mislead it)
+            const int f = warp - 11;
+            int filled = 0;
             bool ok = true;
-            // K stages (and V of 128 dimensions): an instruction is two rows of 256 bytes; V of 256 dimensions: one of 512
+            // wide stages (K, and V of 128 dimensions): an instruction is two rows of 256 bytes; tall ones: one of 512
             const int half = lane >> 4, uk = lane & 15;
-            uint32_t place_k[4], place_v[8];                   // inside a stage, rows 2 j + half, rows j
+            uint32_t wide_at[4], tall_at[8];                   // inside a stage, rows 2 j + half, rows j
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int r = 2 * j + half;
-                place_k[j] = s32(ring) + fw * 4096 + (uk >> 3) * 1024 + r * 128 + (((uk & 7) ^ r) << 4);
+                wide_at[j] = s32(ring) + (uk >> 3) * 1024 + r * 128 + (((uk & 7) ^ r) << 4);
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) place_v[j] = s32(ring) + fw * 8192 + (lane >> 3) * 1024 + j * 128 + (((lane & 7) ^ j) << 4);
-            PageCursor pc[2];                                  // of either half
-            long long off[2], noff[2] = {0, 0};                // elements from the pool to its first row
-            int rows[2], nrows[2] = {0, 0};                    // rows that are there
-            const auto locate = [&](long long (&o)[2], int (&n)[2]) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    int at;
-                    const int page = pc[g].take(at, n[g]);
-                    o[g] = page < 0 ? 0ll : page * P.page_stride + wk.hk * P.head_stride + at * P.tok_stride;
-                }
-            };
-            const auto slot = [&]() {                          // the next stage is free
-                if (rc.wrapped) ok = mbar_wait(s32(&S.empty[rc.idx]), rc.phase ^ 1u, status);
-                ok = __all_sync(0xffffffffu, ok);
-                return ok;
-            };
+            for (int j = 0; j < 8; ++j) tall_at[j] = s32(ring) + (lane >> 3) * 1024 + j * 128 + (((lane & 7) ^ j) << 4);
             const long long two = 2 * P.tok_stride;
-            const auto fetch_wide = [&](const void *pool, const long long (&o)[2], const int (&n)[2], int dim) {   // 128 tokens x 128 dims
-                if (!slot()) return;
-                const uint32_t stage = rc.idx * kStageBytes;
-                const T *const from = static_cast<const T *>(pool) + dim + 8 * uk + half * P.tok_stride;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const T *src = from + o[g];
-                    const bool all = n[g] >= 16;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j, src += two) {
-                        const uint32_t dst = place_k[j & 3] + stage + g * 16384 + (j >> 2) * 2048;
-                        const bool real = all || 2 * j + half < n[g];
-                        copy16(dst, real ? src : static_cast<const T *>(pool), real);
-                    }
-                }
-                arrive_behind_copies(s32(&S.full[rc.idx]));
-                rc.advance(1);
-            };
-            const auto fetch_tall = [&](const void *pool, long long o, int n) {                                     // 64 tokens x 256 dims
-                if (!slot()) return;
-                const uint32_t stage = rc.idx * kStageBytes;
-                const T *src = static_cast<const T *>(pool) + o + 8 * lane;
-                const bool all = n >= 16;
-#pragma unroll
-                for (int j = 0; j < 16; ++j, src += P.tok_stride) {
-                    const bool real = all || j < n;
-                    copy16(place_v[j & 7] + stage + (j >> 3) * 4096, real ? src : static_cast<const T *>(pool), real);
-                }
-                arrive_behind_copies(s32(&S.full[rc.idx]));
-                rc.advance(1);
-            };
+            int skip = 0;                                      // stages of the segment before this warp's first
             while (ok && wk.next()) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g) pc[g].begin(P, wk.b, wk.blk * kTok + 64 * g + 16 * fw, wk.s.len);
-                locate(off, rows);
-                for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, off, rows, h * kDims);
-                for (int i = 0; i < wk.nb && ok; ++i) {
-                    if (i + 1 < wk.nb) {
-                        locate(noff, nrows);
-                        for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, noff, nrows, h * kDims);
+                const int fills = 2 * H * wk.nb;
+                int j = (f + C::kStages - skip) % C::kStages;
+                skip = (skip + fills) % C::kStages;
+                if (j >= fills) continue;
+                const long long head = wk.hk * P.head_stride;
+                Fill fl = fill_of<H>(j, wk.nb);
+                int t = (wk.blk + fl.block) * kTok + 16 * (lane & 7), at;      // lanes 0..7: sixteen tokens each
+                int page = page_of(P, wk.b, t, wk.s.len, at);
+                for (;;) {
+                    const bool there = (unsigned)page < (unsigned)P.num_pages;
+                    const long long off = there ? page * P.page_stride + head + at * P.tok_stride : 0ll;
+                    const int rows = there ? wk.s.len - t : 0;
+                    const Fill now = fl;
+                    const bool more = j + C::kStages < fills;
+                    if (more) {                                // the pages of the warp's next stage
+                        fl = fill_of<H>(j + C::kStages, wk.nb);
+                        t = (wk.blk + fl.block) * kTok + 16 * (lane & 7);
+                        page = page_of(P, wk.b, t, wk.s.len, at);
                     }
-                    if constexpr (H == 2) {
-                        for (int h = 0; h < 2 && ok; ++h) fetch_tall(P.v, off[h], rows[h]);
-                    } else if (ok) {
-                        fetch_wide(P.v, off, rows, 0);
-                    }
+                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const uint32_t stage = f * kStageBytes;
+                    const T *const pool = static_cast<const T *>(now.is_v ? P.v : P.k);
+                    if (H == 2 && now.is_v) {
+#pragma unroll 1
+                        for (int g = 0; g < 4; ++g) {
+                            const T *src = pool + __shfl_sync(0xffffffffu, off, 4 * now.half + g) + 8 * lane;
+                            const int n = __shfl_sync(0xffffffffu, rows, 4 * now.half + g);
+                            if (n >= 16) {
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) { off[g] = noff[g]; rows[g] = nrows[g]; }
+                                for (int i = 0; i < 16; ++i, src += P.tok_stride) copy16(tall_at[i & 7] + stage + g * 8192 + (i >> 3) * 4096, src);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; ++i, src += P.tok_stride)
+                                    copy16(tall_at[i & 7] + stage + g * 8192 + (i >> 3) * 4096, i < n ? src : pool, i < n);
+                            }
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int g = 0; g < 8; ++g) {
+                            const T *src = pool + __shfl_sync(0xffffffffu, off, g) + half * P.tok_stride + now.half * kDims + 8 * uk;
+                            const int n = __shfl_sync(0xffffffffu, rows, g) - half;
+                            if (__all_sync(0xffffffffu, n >= 15)) {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i, src += two) copy16(wide_at[i & 3] + stage + g * 4096 + (i >> 2) * 2048, src);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; ++i, src += two)
+                                    copy16(wide_at[i & 3] + stage + g * 4096 + (i >> 2) * 2048, 2 * i < n ? src : pool, 2 * i < n);
+                            }
+                        }
+                    }
+                    arrive_behind_copies(s32(&(now.is_v ? S.v_full : S.k_full)[f]));
+                    ++filled;
+                    j += C::kStages;
+                    if (!more) break;
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else {
-            // ---------------- e4m3 rows: as above, into raw stages (a warp has 4 KB of one), in instructions of four rows of
-            // 128 bytes, or two of 256; what a thread fetched it widens itself, kRaw - 1 stages later, sixteen bytes into two
-            // units of the swizzled row
-            const int fw = warp - 12;
-            const uint32_t raw = s32(rawring) + fw * 4096 + 16 * lane;
-            const unsigned char *const rawp = rawring + fw * 4096 + 16 * lane;
-            Cursor cc(0, C::kStages);
+            // ---------------- e4m3 rows: warps 2 f and 2 f + 1 fill stage f by way of raw stage f (8 KB each), in instructions of
+            // four rows of 128 bytes, or two of 256
+            const int f = (warp - 11) >> 1, part = (warp - 11) & 1;
+            const uint32_t raw = s32(rawring) + f * kRawBytes + part * 8192 + 16 * lane;
+            const unsigned char *const rawp = rawring + f * kRawBytes + part * 8192 + 16 * lane;
             bool ok = true;
-            int issued = 0, done = 0;
-            uint32_t tall = 0;                                 // bit s % kRaw: raw stage s is 64 tokens x 256 bytes
-            const auto widen = [&]() {
-                if (cc.wrapped) ok = mbar_wait(s32(&S.empty[cc.idx]), cc.phase ^ 1u, status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) return;
-                const int rs = done % C::kRaw;
-                const unsigned char *const src = rawp + rs * kRawBytes;
-                unsigned char *const dst = ring + cc.idx * kStageBytes;
-                const bool is_tall = H == 2 && (tall >> rs & 1);
-                const int sub = is_tall ? lane >> 4 : lane >> 3, u = is_tall ? lane & 15 : lane & 7;      // row of the instruction, piece of the row
-                const bool swap = u & 4;                       // lanes of a row start with different units: no bank conflicts
-                const int k0 = (u & 3) * 2 + (swap ? 1 : 0), k1 = (u & 3) * 2 + (swap ? 0 : 1);
+            int filled = 0;
+            // rows and pieces of a wide instruction (four rows of eight pieces) and a tall one (two of sixteen); a piece is two
+            // units of the swizzled row, and the lanes of a row start with different ones: no bank conflicts
+            const int wsub = lane >> 3, wu = lane & 7, tsub = lane >> 4, tu = lane & 15;
+            const bool swap = lane & 4;
+            uint32_t wide_at[2], tall_at[4];                   // rows 4 j + wsub, 2 j + tsub of an atom
 #pragma unroll
-                for (int b = 0; b < 8; b += 4) {
-                    uint4 x[4];
+            for (int j = 0; j < 2; ++j) {
+                const int r = 4 * j + wsub;
+                wide_at[j] = (wu >> 2) * 1024 + r * 128 + ((((wu & 3) * 2 + (swap ? 1 : 0)) ^ r) << 4);
+            }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4 *>(src + 512 * (b + j));
+            for (int j = 0; j < 4; ++j) {
+                const int r = 2 * j + tsub;
+                tall_at[j] = (tu >> 2) * 1024 + r * 128 + ((((tu & 3) * 2 + (swap ? 1 : 0)) ^ r) << 4);
+            }
+            // fetch quarter b of this warp's part of a stage (sixteen tokens wide, or eight tall): four instructions
+            const auto fetch = [&](const Fill &fl, long long off, int rows, int b) {
+                const unsigned char *const pool = static_cast<const unsigned char *>(fl.is_v ? P.v : P.k);
+                const bool tall = H == 2 && fl.is_v;
+                const int lane_of = tall ? 4 * fl.half + 2 * part + (b >> 1) : 4 * part + b;    // whose page it is
+                const int row0 = tall ? (b & 1) * 8 + tsub : wsub, inc = tall ? 2 : 4;
+                const unsigned char *src = pool + __shfl_sync(0xffffffffu, off, lane_of) + row0 * P.tok_stride + (tall ? 16 * tu : fl.half * kDims + 16 * wu);
+                const int n = __shfl_sync(0xffffffffu, rows, lane_of) - row0;
+                const long long step = inc * P.tok_stride;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // row of the stage: tall 16 fw + 2 i + sub; else 64 (i / 4) + 16 fw + 4 (i % 4) + sub
-                        const int i = b + j, r = is_tall ? 16 * fw + 2 * i + sub : 64 * (i >> 2) + 16 * fw + 4 * (i & 3) + sub;
-                        uint4 a, c;
-                        widen4<T>(x[j].x, a.x, a.y);
-                        widen4<T>(x[j].y, a.z, a.w);
-                        widen4<T>(x[j].z, c.x, c.y);
-                        widen4<T>(x[j].w, c.z, c.w);
-                        unsigned char *const at = dst + (r >> 3) * (is_tall ? 4096 : 2048) + (u >> 2) * 1024 + (r & 7) * 128;
-                        *reinterpret_cast<uint4 *>(at + ((k0 ^ (r & 7)) << 4)) = swap ? c : a;
-                        *reinterpret_cast<uint4 *>(at + ((k1 ^ (r & 7)) << 4)) = swap ? a : c;
-                    }
-                }
-                fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(s32(&S.full[cc.idx]));
-                ++done;
-                cc.advance(1);
-            };
-            PageCursor pc[2];
-            long long off[2], noff[2] = {0, 0};
-            int rows[2], nrows[2] = {0, 0};
-            const auto locate = [&](long long (&o)[2], int (&n)[2]) {
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    int at;
-                    const int page = pc[g].take(at, n[g]);
-                    o[g] = page < 0 ? 0ll : page * P.page_stride + wk.hk * P.head_stride + at * P.tok_stride;
+                for (int i = 0; i < 4; ++i, src += step) {
+                    const bool real = inc * i < n;
+                    copy16(raw + b * 2048 + i * 512, real ? src : pool, real);
                 }
             };
-            const auto issue = [&](bool is_tall) {
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                tall = (tall & ~(1u << issued % C::kRaw)) | (is_tall ? 1u : 0u) << issued % C::kRaw;
-                ++issued;
-                if (issued >= C::kRaw) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(C::kRaw - 1) : "memory");
-                    widen();
-                }
-            };
-            const long long two = 2 * P.tok_stride, four = 4 * P.tok_stride;
-            const auto fetch_wide = [&](const void *pool, const long long (&o)[2], const int (&n)[2], int dim) {
-                const uint32_t to = raw + (issued % C::kRaw) * kRawBytes;
-                const int sub = lane >> 3;
-                const unsigned char *const from = static_cast<const unsigned char *>(pool) + dim + 16 * (lane & 7) + sub * P.tok_stride;
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    const unsigned char *src = from + o[g];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j, src += four) {
-                        const bool real = 4 * j + sub < n[g];
-                        copy16(to + 512 * (4 * g + j), real ? src : static_cast<const unsigned char *>(pool), real);
-                    }
-                }
-                issue(false);
-            };
-            const auto fetch_tall = [&](const void *pool, long long o, int n) {
-                const uint32_t to = raw + (issued % C::kRaw) * kRawBytes;
-                const int sub = lane >> 4;
-                const unsigned char *src = static_cast<const unsigned char *>(pool) + o + 16 * (lane & 15) + sub * P.tok_stride;
-#pragma unroll
-                for (int j = 0; j < 8; ++j, src += two) {
-                    const bool real = 2 * j + sub < n;
-                    copy16(to + 512 * j, real ? src : static_cast<const unsigned char *>(pool), real);
-                }
-                issue(true);
-            };
+            int skip = 0;
             while (ok && wk.next()) {
+                const int fills = 2 * H * wk.nb;
+                int j = (f + C::kStages - skip) % C::kStages;
+                skip = (skip + fills) % C::kStages;
+                if (j >= fills) continue;
+                const long long head = wk.hk * P.head_stride;
+                Fill fl = fill_of<H>(j, wk.nb);
+                int t, at, page, rows = 0;
+                long long off = 0;
+                const auto look = [&]() {                      // lanes 0..7: the page of sixteen tokens each
+                    t = (wk.blk + fl.block) * kTok + 16 * (lane & 7);
+                    page = page_of(P, wk.b, t, wk.s.len, at);
+                };
+                const auto place = [&]() {
+                    const bool there = (unsigned)page < (unsigned)P.num_pages;
+                    off = there ? page * P.page_stride + head + at * P.tok_stride : 0ll;
+                    rows = there ? wk.s.len - t : 0;
+                };
+                look();
+                place();
+#pragma unroll 1
+                for (int b = 0; b < 4; ++b) fetch(fl, off, rows, b);
+                for (;;) {
+                    const Fill now = fl;
+                    const bool more = j + C::kStages < fills;
+                    if (more) { fl = fill_of<H>(j + C::kStages, wk.nb); look(); }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (more) place();
+                    unsigned char *const dst = ring + f * kStageBytes + part * 16384;
+                    const bool tall = H == 2 && now.is_v;
+#pragma unroll 1
+                    for (int b = 0; b < 4; ++b) {
+                        uint4 x[4];
 #pragma unroll
-                for (int g = 0; g < 2; ++g) pc[g].begin(P, wk.b, wk.blk * kTok + 64 * g + 16 * fw, wk.s.len);
-                locate(off, rows);
-                for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, off, rows, h * kDims);
-                for (int i = 0; i < wk.nb && ok; ++i) {
-                    if (i + 1 < wk.nb) {
-                        locate(noff, nrows);
-                        for (int h = 0; h < H && ok; ++h) fetch_wide(P.k, noff, nrows, h * kDims);
-                    }
-                    if constexpr (H == 2) {
-                        for (int h = 0; h < 2 && ok; ++h) fetch_tall(P.v, off[h], rows[h]);
-                    } else if (ok) {
-                        fetch_wide(P.v, off, rows, 0);
-                    }
+                        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4 *>(rawp + b * 2048 + i * 512);
 #pragma unroll
-                    for (int g = 0; g < 2; ++g) { off[g] = noff[g]; rows[g] = nrows[g]; }
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 lo, hi;
+                            widen4<T>(x[i].x, lo.x, lo.y);
+                            widen4<T>(x[i].y, lo.z, lo.w);
+                            widen4<T>(x[i].z, hi.x, hi.y);
+                            widen4<T>(x[i].w, hi.z, hi.w);
+                            // wide: rows 16 b + 4 i + wsub of 64; tall: 8 b + 2 i + tsub of 32
+                            const uint32_t to = tall ? tall_at[i] + b * 4096 : wide_at[i & 1] + b * 4096 + (i >> 1) * 2048;
+                            *reinterpret_cast<uint4 *>(dst + to) = swap ? hi : lo;
+                            *reinterpret_cast<uint4 *>(dst + (to ^ 16)) = swap ? lo : hi;
+                        }
+                        if (more) fetch(fl, off, rows, b);     // these pieces of the raw stage are in registers, and done with
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s32(&(now.is_v ? S.v_full : S.k_full)[f]));
+                    ++filled;
+                    j += C::kStages;
+                    if (!more) break;
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-            while (ok && done < issued) widen();
         }
     }
     fence_before_sync();
@@ -1021,7 +1042,7 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     P.batch = batch; P.tokens = tokens; P.max_drafts = max_drafts; P.kvh = kvh; P.G = q_heads / kvh; P.tiles = z.tiles;
     const float s2 = scale * cache->k_scale * 1.4426950408889634f;
     P.negate = s2 < 0.f;
-    P.scale_log2 = P.negate ? -s2 : s2;
+    P.scale_log2 = fmaxf(P.negate ? -s2 : s2, 1e-37f);       // (zero times the minus infinity of an unseen token would be NaN)
     P.v_scale = cache->v_scale;
     P.rows_ws = z.rows_ws;
     P.plan = (int *)workspace;
