@@ -396,7 +396,7 @@ int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out, long long
  *   seq_lens     int32 [batch], drafts included; starts int32 [batch + 1], ascending; mask int64 [tokens] or NULL
  *   max_drafts   1 .. EXL3_TREE_MAX_DRAFTS, the largest number of drafts of a sequence; rows of a sequence from
  *                max_drafts on are not computed
- *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads, at most 64 times as many
+ *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads, at most 32 times as many
  *   workspace    exl3_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, need not be cleared; calls that share it
  *                must not overlap on the device
  * K and V are read at 16 bits (e4m3 widened exactly), scores, statistics and sums are fp32, the probabilities are

@@ -51,7 +51,7 @@ constexpr int kTok = 128;                     // tokens of a block
 constexpr int kDims = 128;                    // dimensions of a stage
 constexpr int kStageBytes = kTok * kDims * 2; // 32 KB
 constexpr int kRawBytes = kTok * kDims;       // 16 KB of e4m3
-constexpr int kMaxTiles = 32;
+constexpr int kMaxTiles = 16;
 constexpr int kMaxGrid = 148;
 constexpr float kRaise = 8.f;                 // log2 units the maximum may lag behind
 
@@ -70,7 +70,8 @@ struct Params {
     float scale_log2, v_scale;
     int negate;                               // the scale is negative: Q K^T is negated, scale_log2 is its size
     int rows_ws;                              // rows of a partial result (a multiple of 32)
-    int *plan;                                // [0..32) CTAs per tile, [32..64) blocks per tile, then per tile [batch + 1] prefix sums
+    int4 *joins;                              // per CTA: the pair whose blocks begin in its piece and end behind it: (sequence,
+                                              // KV head, parts, tile * 2 + slot of the first part); x < 0: none
     float *part_ml, *part_o;                  // [2 * grid][2][rows_ws], [2 * grid][HD / 4][rows_ws][4]: lane = row, full lines
 };
 
@@ -82,8 +83,7 @@ struct Shared {
     uint32_t tmem_base;
     int nonfinite[2];                         // of the current segment and the one before, in turn
     float top[kM], sum[2][kM];                // of the rows; sums of the two groups
-    int total[kMaxTiles];
-    int sums[20];                             // one per warp
+    int part[kMaxTiles][20];                  // blocks per tile and warp
     int first_seq, first_off;
 };
 static_assert(sizeof(Shared) <= 3072, "shared state");
@@ -221,10 +221,10 @@ struct Walk {
 };
 
 // CTAs of tile `lane` out of `grid`, in proportion to its blocks (at least one).  Tiles of equal work get equal numbers,
-// so that their CTAs walk the same blocks at the same time.  A whole warp; totals[0] is the largest.
-__device__ __forceinline__ int share_of(const int *totals, int tiles, int grid, int lane) {
-    if (tiles == 1) return lane == 0 && totals[0] ? grid : 0;
-    const double u = lane < tiles ? totals[lane] : 0;
+// so that their CTAs walk the same blocks at the same time.  A whole warp; the first tile has the most blocks.
+__device__ __forceinline__ int share_of(int blocks, int tiles, int grid, int lane) {
+    if (tiles == 1) return lane == 0 && blocks ? grid : 0;
+    const double u = blocks;
     double all = u;
 #pragma unroll
     for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
@@ -301,7 +301,6 @@ tree_attn_kernel(const __grid_constant__ Params P) {
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async();
     }
-    if (tid < kMaxTiles) S.total[tid] = 0;
     if (warp == 1) tmem_alloc(s32(&S.tmem_base), 512);
     fence_before_sync();
     __syncthreads();
@@ -310,58 +309,63 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     asm volatile("griddepcontrol.wait;" ::: "memory");       // lengths, queries, cache rows of the kernels before
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // ---- this CTA's piece of the line
-    for (int b0 = 0; b0 < P.batch; b0 += kThreads) {
-        const int b = b0 + tid;
-        int rows = 0, count = 0;
-        if (b < P.batch) { const Seq s = seq_of(P, b); rows = s.rows; count = s.blocks * P.kvh; }
-        for (int m = 0; m < P.tiles; ++m) {
-            const int sum = __reduce_add_sync(0xffffffffu, rows > kM * m ? count : 0);
-            if (lane == 0 && sum) atomicAdd(&S.total[m], sum);
-        }
+    // ---- this CTA's piece of the line: a thread has a run of sequences
+    constexpr int kWarps = kThreads / 32;
+    const int run = (P.batch + kThreads - 1) / kThreads, b0 = tid * run, b1 = min(P.batch, b0 + run);
+    Seq s0 = {};
+    if (b0 < b1) s0 = seq_of(P, b0);
+    const auto blocks_of = [&](int m) {                      // of the run, in tile m
+        int v = s0.rows > kM * m ? s0.blocks * P.kvh : 0;
+        for (int b = b0 + 1; b < b1; ++b) { const Seq s = seq_of(P, b); v += s.rows > kM * m ? s.blocks * P.kvh : 0; }
+        return v;
+    };
+    for (int t = 0; t < P.tiles; ++t) {
+        const int sum = __reduce_add_sync(0xffffffffu, blocks_of(t));
+        if (lane == 0) S.part[t][warp] = sum;
     }
+    if (tid == 0) P.joins[blockIdx.x] = make_int4(-1, 0, 0, 0);
     __syncthreads();
-    int m = 0, w = blockIdx.x, W = 0;
+    int m = 0, w = blockIdx.x, W = 0, U = 0;
     {
-        const int mine = share_of(S.total, P.tiles, gridDim.x, lane);
-        int upto = mine;                                     // CTAs of the tiles up to this lane's
+        int mine = 0;                                        // lane = tile: its blocks
+        if (lane < P.tiles)
+            for (int i = 0; i < kWarps; ++i) mine += S.part[lane][i];
+        const int share = share_of(mine, P.tiles, gridDim.x, lane);
+        int upto = share;                                    // CTAs of the tiles up to this lane's
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += y;
         }
         const uint32_t behind = __ballot_sync(0xffffffffu, upto > (int)blockIdx.x);
-        m = behind ? __ffs(behind) - 1 : 0;
-        W = __shfl_sync(0xffffffffu, behind ? mine : 0, m);
-        w -= __shfl_sync(0xffffffffu, upto - mine, m);
-        if (blockIdx.x == 0 && tid < P.tiles) { P.plan[tid] = mine; P.plan[kMaxTiles + tid] = S.total[tid]; }
+        if (behind) {
+            m = __ffs(behind) - 1;
+            W = __shfl_sync(0xffffffffu, share, m);
+            U = __shfl_sync(0xffffffffu, mine, m);
+            w -= __shfl_sync(0xffffffffu, upto - share, m);
+        }
     }
-    const int u0 = W ? piece(S.total[m], W, w) : 0, u1 = W ? piece(S.total[m], W, w + 1) : 0;
-    if (W && (u1 > u0 || w == 0)) {
-        int carry = 0;
-        for (int b0 = 0; b0 < P.batch; b0 += kThreads) {
-            const int b = b0 + tid;
-            int v = 0;
-            if (b < P.batch) { const Seq s = seq_of(P, b); v = s.rows > kM * m ? s.blocks * P.kvh : 0; }
-            int x = v;
+    const int u0 = W ? piece(U, W, w) : 0, u1 = W ? piece(U, W, w + 1) : 0;
+    if (u1 > u0) {                                           // whose run holds the first block?
+        const int v = blocks_of(m);
+        int x = v;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        int off = u0 - (x - v);
+        for (int i = 0; i < warp; ++i) off -= S.part[m][i];
+        if (off >= 0 && off < v) {
+            int b = b0;
+            for (Seq s = s0;; s = seq_of(P, b)) {
+                const int n = s.rows > kM * m ? s.blocks * P.kvh : 0;
+                if (off < n) break;
+                off -= n;
+                ++b;
             }
-            if (b0) __syncthreads();
-            if (lane == 31) S.sums[warp] = x;
-            __syncthreads();
-            int before = carry, all = 0;
-            for (int i = 0; i < kThreads / 32; ++i) { if (i < warp) before += S.sums[i]; all += S.sums[i]; }
-            const int excl = before + x - v;
-            if (v && u0 >= excl && u0 < excl + v) { S.first_seq = b; S.first_off = u0 - excl; }
-            if (w == 0) {
-                int *const prefix = P.plan + 2 * kMaxTiles + (size_t)m * (P.batch + 1);
-                if (b < P.batch) prefix[b] = excl;
-                if (b == P.batch - 1) prefix[P.batch] = excl + v;
-            }
-            carry += all;
+            S.first_seq = b;
+            S.first_off = off;
         }
     }
     __syncthreads();
@@ -492,7 +496,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
             // garbage then, the status word says so).
             bool ok = true;
             const auto hold = [&](uint64_t *bar, uint32_t parity) {
-                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s32(bar), parity, status));
+                if (ok) ok = __all_sync(0xffffffffu, mbar_wait(s32(bar), parity, status, 40));
                 fence_after_sync();
             };
             int cnt = 0, pos = 0;                              // blocks done; ring position of the segment
@@ -505,6 +509,30 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 if (live) bits = P.mask ? (unsigned long long)__ldg(P.mask + wk.s.first + draft) : (draft >= 63 ? ~0ull : (2ull << draft) - 1);
                 float top = -INFINITY;
                 float2 sum2 = make_float2(0.f, 0.f);           // over this group's blocks, relative to `top`
+                // Non-finite values of drafts in V become zeros (see the top of the file).
+                const auto clean = [&](int n, int i, int tok0) {
+                    if (tok0 + kTok <= ctx) return;
+                    const int from = max(0, ctx - tok0), upto = min(kTok, wk.s.len - tok0);
+                    const int vpos = pos + H + 2 * H * i + (i + 1 < wk.nb ? H : 0);
+                    hold(&S.v_here[n & 1], (n >> 1) & 1);      // (announced by the MMA thread, which looks at every stage in its turn)
+                    constexpr int kUnits = HD / 8, kRowsV = kTok / H;           // 16-byte units of a row, rows of a stage
+                    for (int e = row; e < (upto - from) * kUnits; e += 128) {
+                        const int r = from + e / kUnits, u = e % kUnits, st = (vpos + r / kRowsV) % C::kStages, q = r % kRowsV;
+                        uint4 *const at = reinterpret_cast<uint4 *>(ring + (size_t)st * kStageBytes + (q >> 3) * (HD * 16) + (u >> 3) * 1024 +
+                                                                    (q & 7) * 128 + (((u & 7) ^ (q & 7)) << 4));
+                        const uint4 v = *at;
+                        uint4 y;
+                        const bool a = nonfinite2<T>(v.x, y.x), b2 = nonfinite2<T>(v.y, y.y), c = nonfinite2<T>(v.z, y.z),
+                                   d = nonfinite2<T>(v.w, y.w);
+                        if (a || b2 || c || d) { *at = y; S.nonfinite[wk.index & 1] = 1; }
+                    }
+                    fence_async();
+                };
+                const auto ready = [&](int n) {
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(s32(&S.p_ready[n & 1]));
+                };
                 for (int i = (cnt ^ side) & 1; i < wk.nb; i += 2) {
                     const int n = cnt + i, tok0 = (wk.blk + i) * kTok;         // n: number of the block in the CTA
                     int at;
@@ -523,9 +551,12 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         return live ? v : 0u;
                     };
                     // (The loops over four times 32 scores stay loops: unrolled, the code of the roles did not fit the instruction
-                    // caches, and the warps waited for instructions more often than for anything else but loads.)
+                    // caches, and the warps waited for instructions more often than for anything but loads.  Nor did it pay to take
+                    // the exponentials against the maximum known so far and read the scores once: 85 against 79 us at 61 drafts over
+                    // 32768 tokens, the probabilities being in registers until that maximum is confirmed, and the loop unrolled.)
+                    const uint32_t s_t = tmem + lane_base + HD + (n & 1) * kTok;
                     const auto load = [&](int k, uint32_t (&y)[32]) {          // scores, minus infinity where nothing is seen
-                        tmem_ld32(tmem + lane_base + HD + (n & 1) * kTok + 32 * k, y);
+                        tmem_ld32(s_t + 32 * k, y);
                         const uint32_t vis = masked ? seen(k) : ~0u;
                         tmem_wait_ld();
                         if (masked) {
@@ -533,8 +564,12 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                             for (int e = 0; e < 32; ++e) y[e] = vis >> e & 1 ? y[e] : 0xFF800000u;
                         }
                     };
-                    const uint32_t s_t = tmem + lane_base + HD + (n & 1) * kTok;
                     hold(&S.s_full[n & 1], (n >> 1) & 1);
+                    if (32 * quarter >= rows) {                // no rows in this quarter: whatever lies there as P stays in its lanes
+                        clean(n, i, tok0);
+                        ready(n);
+                        continue;
+                    }
                     float mx = -INFINITY;
 #pragma unroll 1
                     for (int k = 0; k < 4; ++k) {
@@ -546,7 +581,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                     }
                     mx = mx == -INFINITY ? mx : mx * P.scale_log2;
-                    if (i > 0) {                               // the maximum as the block before left it
+                    if (i > 0) {                               // the maximum as the block before left it, and this group's sum with it
                         take_over(1 + 4 * (side ^ 1) + quarter);
                         const float before = top;
                         top = S.top[row];
@@ -585,29 +620,9 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         }
                         tmem_st16(s_t + 16 * k, p);            // over scores that were read
                     }
-                    if (tok0 + kTok > ctx) {
-                        // non-finite values of drafts become zeros (see the top of the file)
-                        const int from = max(0, ctx - tok0), upto = min(kTok, wk.s.len - tok0);
-                        const int vpos = pos + H + 2 * H * i + (i + 1 < wk.nb ? H : 0);
-                        // (announced by the MMA thread, which looks at every stage in its turn)
-                        hold(&S.v_here[n & 1], (n >> 1) & 1);
-                        constexpr int kUnits = HD / 8, kRowsV = kTok / H;           // 16-byte units of a row, rows of a stage
-                        for (int e = row; e < (upto - from) * kUnits; e += 128) {
-                            const int r = from + e / kUnits, u = e % kUnits, st = (vpos + r / kRowsV) % C::kStages, q = r % kRowsV;
-                            uint4 *const at = reinterpret_cast<uint4 *>(ring + (size_t)st * kStageBytes + (q >> 3) * (HD * 16) + (u >> 3) * 1024 +
-                                                                        (q & 7) * 128 + (((u & 7) ^ (q & 7)) << 4));
-                            const uint4 v = *at;
-                            uint4 y;
-                            const bool a = nonfinite2<T>(v.x, y.x), b2 = nonfinite2<T>(v.y, y.y), c = nonfinite2<T>(v.z, y.z),
-                                       d = nonfinite2<T>(v.w, y.w);
-                            if (a || b2 || c || d) { *at = y; S.nonfinite[wk.index & 1] = 1; }
-                        }
-                        fence_async();
-                    }
+                    clean(n, i, tok0);
                     tmem_wait_st();
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(s32(&S.p_ready[n & 1]));
+                    ready(n);
                 }
                 // ---- the segment's result
                 cnt += wk.nb;
@@ -691,6 +706,11 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     }
                     __syncwarp();
                 }
+                if (!whole && wk.blk == 0 && tid == 96) {          // more parts follow in the next CTAs
+                    const int q = U / W, r = U - q * W, last = u1 + wk.nblk - wk.nb - 1;     // the pair's last block
+                    const int owner = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
+                    P.joins[blockIdx.x] = make_int4(wk.b, wk.hk, owner - w + 1, 2 * m + (wk.index ? 1 : 0));
+                }
                 if (live && !whole && side == 0) {
                     P.part_ml[(size_t)(2 * slot) * P.rows_ws + row] = top;
                     P.part_ml[(size_t)(2 * slot + 1) * P.rows_ws + row] = sum;
@@ -738,7 +758,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         t = (wk.blk + fl.block) * kTok + 16 * (lane & 7);
                         page = page_of(P, wk.b, t, wk.s.len, at);
                     }
-                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status);
+                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status, 40);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     const uint32_t stage = f * kStageBytes;
@@ -845,7 +865,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     const bool more = j + C::kStages < fills;
                     if (more) { fl = fill_of<H>(j + C::kStages, wk.nb); look(); }
                     asm volatile("cp.async.wait_all;" ::: "memory");
-                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status);
+                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status, 40);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     if (more) place();
@@ -899,28 +919,13 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int row0 = blockIdx.y / (HD / kMergeCols) * 32, col0 = blockIdx.y % (HD / kMergeCols) * kMergeCols;
-    int m = 0, cta0 = 0;
-    while (m < P.tiles && (int)blockIdx.x >= cta0 + P.plan[m]) cta0 += P.plan[m++];
-    if (m >= P.tiles) return;
-    const int W = P.plan[m], U = P.plan[kMaxTiles + m], w = blockIdx.x - cta0;
-    const int u0 = piece(U, W, w), u1 = piece(U, W, w + 1);
-    if (u1 <= u0 || w + 1 >= W) return;
-    const int *const prefix = P.plan + 2 * kMaxTiles + (size_t)m * (P.batch + 1);
-    int lo = 0, hi = P.batch - 1;
-    while (lo < hi) {                                          // last sequence that begins at or before the piece's last block
-        const int mid = (lo + hi + 1) >> 1;
-        if (prefix[mid] <= u1 - 1) lo = mid; else hi = mid - 1;
-    }
-    const int b = lo, base = prefix[b], nblk = (prefix[b + 1] - base) / P.kvh;
-    if (nblk <= 0) return;
-    const int hk = (u1 - 1 - base) / nblk, begin = base + hk * nblk, end = begin + nblk;
-    if (begin < u0 || end <= u1) return;
+    const int4 join = P.joins[blockIdx.x];
+    if (join.x < 0) return;
+    const int b = join.x, hk = join.y, parts = join.z, m = join.w >> 1;
     const Seq s = seq_of(P, b);
     const int rows = min(kM, s.rows - kM * m) - row0;          // of these 32
     if (rows <= 0) return;
-    int parts = 2;                                             // the CTAs w .. w + parts - 1 hold blocks of it
-    while (w + parts < W && piece(U, W, w + parts) < end) ++parts;
-    const int first = 2 * (cta0 + w) + (begin != u0 ? 1 : 0), next = 2 * (cta0 + w + 1);     // slots: first, next, next + 2, ..
+    const int first = 2 * blockIdx.x + (join.w & 1), next = 2 * (blockIdx.x + 1);       // slots: first, next, next + 2, ..
     const int row = row0 + min(lane, rows - 1);
     const auto slot = [&](int k) { return (size_t)(k ? next + 2 * (k - 1) : first); };
     float top = -INFINITY;
@@ -955,15 +960,15 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
 }
 
 // ---------------------------------------------------------------- host side
-struct Sizes { int tiles, rows_ws; size_t plan, ml, total; };
-static Sizes sizes_of(int batch, int G, int max_drafts, int hd) {
+struct Sizes { int tiles, rows_ws; size_t joins, ml, total; };
+static Sizes sizes_of(int G, int max_drafts, int hd) {
     Sizes z;
     const int rows = max_drafts * G;
     z.tiles = (rows + kM - 1) / kM;
     z.rows_ws = rows < kM ? (rows + 31) / 32 * 32 : kM;
-    z.plan = ((size_t)(2 * kMaxTiles + (size_t)z.tiles * (batch + 1)) * 4 + 255) & ~(size_t)255;
+    z.joins = (kMaxGrid * sizeof(int4) + 255) & ~(size_t)255;
     z.ml = ((size_t)2 * kMaxGrid * z.rows_ws * 8 + 255) & ~(size_t)255;
-    z.total = z.plan + z.ml + (size_t)2 * kMaxGrid * z.rows_ws * hd * 4;
+    z.total = z.joins + z.ml + (size_t)2 * kMaxGrid * z.rows_ws * hd * 4;
     return z;
 }
 
@@ -1004,7 +1009,7 @@ extern "C" size_t exl3_tree_attn_workspace_bytes(int batch, int q_heads, int max
     if (!cache || batch <= 0 || q_heads <= 0 || cache->kv_heads <= 0 || q_heads % cache->kv_heads || max_drafts < 1 ||
         max_drafts > EXL3_TREE_MAX_DRAFTS || (cache->head_dim != 128 && cache->head_dim != 256))
         return 0;
-    return exl3::tree::sizes_of(batch, q_heads / cache->kv_heads, max_drafts, cache->head_dim).total;
+    return exl3::tree::sizes_of(q_heads / cache->kv_heads, max_drafts, cache->head_dim).total;
 }
 
 extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long long out_stride, const void *block_table,
@@ -1024,12 +1029,12 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
         max_drafts < 1 || max_drafts > EXL3_TREE_MAX_DRAFTS ||
         (long long)batch * kvh * (((long long)table_width * cache->page_size + kTok - 1) / kTok + 1) > INT_MAX)
         return EXL3_E_SHAPE;
-    if (q_heads / kvh > 64) return EXL3_E_UNSUPPORTED;
+    if (q_heads / kvh > 2 * kMaxTiles) return EXL3_E_UNSUPPORTED;      // 64 drafts of as many heads are kMaxTiles tiles
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(starts, 4) ||
         !aligned(mask, 8))
         return EXL3_E_ALIGN;
     if (batch == 0 || tokens == 0) return EXL3_OK;
-    const Sizes z = sizes_of(batch, q_heads / kvh, max_drafts, hd);
+    const Sizes z = sizes_of(q_heads / kvh, max_drafts, hd);
     if (!workspace || workspace_bytes < z.total) return EXL3_E_WORKSPACE;
     if (!aligned(workspace, 16)) return EXL3_E_ALIGN;
     Params P = {};
@@ -1045,9 +1050,9 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     P.scale_log2 = fmaxf(P.negate ? -s2 : s2, 1e-37f);       // (zero times the minus infinity of an unseen token would be NaN)
     P.v_scale = cache->v_scale;
     P.rows_ws = z.rows_ws;
-    P.plan = (int *)workspace;
-    P.part_ml = (float *)((char *)workspace + z.plan);
-    P.part_o = (float *)((char *)workspace + z.plan + z.ml);
+    P.joins = (int4 *)workspace;
+    P.part_ml = (float *)((char *)workspace + z.joins);
+    P.part_o = (float *)((char *)workspace + z.joins + z.ml);
     const bool fp8 = cache->dtype == EXL3_KV_E4M3;
     cudaStream_t st = (cudaStream_t)stream;
     if (hd == 256) {
