@@ -438,9 +438,10 @@ typedef struct exl3_page_tables {
     int table_stride, table_width, max_seqs, num_pages, page_size;
 } exl3_page_tables;
 typedef struct exl3_page_pools {
-    void *const *pools;                 /* host array of num_pools device pointers */
+    void *const *pools;                 /* host array of num_pools device pointers, or of one (pool_stride) */
     long long page_stride, head_stride, token_stride;    /* bytes */
     int num_pools, heads, row_bytes;    /* row_bytes: one token of one head, at most 1024 */
+    long long pool_stride;              /* 0, or: pool i lies i * pool_stride bytes behind pools[0] */
 } exl3_page_pools;
 /*
  * children[i] (which hold nothing) become copies of parents[i]: full pages are shared, the used rows of a partial last

@@ -423,10 +423,12 @@ static int read_pools(const exl3_page_pools *in, PoolList &l, RowGeom &g) {
         in->row_bytes > 1024 || in->heads > 65535 || in->page_stride <= 0 || in->head_stride < in->row_bytes ||
         in->token_stride < in->row_bytes || (in->page_stride & 15) || (in->head_stride & 15) || (in->token_stride & 15))
         return EXL3_E_SHAPE;
+    if (in->pool_stride < 0 || (in->pool_stride & 15)) return EXL3_E_SHAPE;
     for (int i = 0; i < in->num_pools; ++i) {
-        if (!in->pools[i]) return EXL3_E_NULL;
-        if (!aligned(in->pools[i], 16)) return EXL3_E_ALIGN;
-        l.pool[i] = in->pools[i];
+        void *const p = in->pool_stride ? (in->pools[0] ? (char *)in->pools[0] + i * in->pool_stride : nullptr) : in->pools[i];
+        if (!p) return EXL3_E_NULL;
+        if (!aligned(p, 16)) return EXL3_E_ALIGN;
+        l.pool[i] = p;
     }
     g = RowGeom{in->page_stride, in->head_stride, in->token_stride, in->heads, in->row_bytes};
     return EXL3_OK;

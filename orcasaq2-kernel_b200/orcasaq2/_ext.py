@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 import warnings
 
@@ -104,8 +105,7 @@ def lib():
                 L.exl3_decode_attn_paged_fp8.restype = ci
                 L.exl3_rope_append_fp8.argtypes = [vp, ci, vp, vp, ci, vp, vp, ci, ci, ci, ci, ci, ll, ll, cf, cf, vp]
                 L.exl3_rope_append_fp8.restype = ci
-                pc = ctypes.POINTER(Exl3PagedCache)
-                pt, pp = ctypes.POINTER(Exl3PageTables), ctypes.POINTER(Exl3PagePools)
+                pc = pt = pp = vp                     # structs: by address, or packed into bytes
                 L.exl3_qk_norm_rope_append.argtypes = [vp, ll, vp, ll, vp, vp, ci, cf, vp, vp, ci, ci, ci, vp, vp, ci, ci,
                                                        ci, pc, vp]
                 L.exl3_qk_norm_rope_append.restype = ci
@@ -630,7 +630,7 @@ class Exl3PageTables(ctypes.Structure):
 class Exl3PagePools(ctypes.Structure):
     _fields_ = [("pools", ctypes.POINTER(ctypes.c_void_p)), ("page_stride", ctypes.c_longlong),
                 ("head_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong), ("num_pools", ctypes.c_int),
-                ("heads", ctypes.c_int), ("row_bytes", ctypes.c_int)]
+                ("heads", ctypes.c_int), ("row_bytes", ctypes.c_int), ("pool_stride", ctypes.c_longlong)]
 
 
 TREE_MAX_DRAFTS = 64
@@ -645,44 +645,60 @@ def _need(ok: bool, what: str):
         raise RuntimeError(what)
 
 
-def _call(dev: torch.device, fn, *args):
-    """fn(*args, stream): the current stream of `dev`, with `dev` current while it launches."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+# The calls below are made for every layer and step, and often take the GPU less time than the host: structs are packed
+# into bytes (a tenth of a ctypes.Structure's cost), and tensors are looked at no more than it takes to refuse a wrong one.
+_PACK_CACHE = struct.Struct("@PPqqqiiiiiff").pack
+_PACK_TABLES = struct.Struct("@PPPPPPiiiii").pack
+_PACK_POOLS = struct.Struct("@Pqqqiii4xq").pack
+_I32, _I64 = torch.int32, torch.int64
+
+
+def _call(idx: int, fn, *args):
+    """fn(*args, stream): the current stream of CUDA device `idx`, with that device current while it launches."""
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
     if rc:
         _check(rc, fn.__name__)
 
 
-def _ints(t, name: str, dev: torch.device, dtype=torch.int32, dim: int = 1):
-    if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != dtype or t.dim() != dim or \
-            (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise RuntimeError(f"{name} must be a {dim}-D {dtype} tensor on {dev} with contiguous rows")
-    return t
+def _ints(t, name: str, idx: int, dtype=_I32, dim: int = 1):
+    if not isinstance(t, torch.Tensor) or t.get_device() != idx or t.dtype is not dtype or t.dim() != dim or \
+            (t.stride(-1) != 1 and t.shape[-1] > 1):
+        raise RuntimeError(f"{name} must be a {dim}-D {dtype} tensor on CUDA device {idx} with contiguous rows")
+    return t.data_ptr()
 
 
-def _paged(name: str, x: torch.Tensor, k, v, layout: str, k_scale: float, v_scale: float) -> Exl3PagedCache:
-    """The description of the page pools that the C entry points take; x holds the 16-bit values beside them."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
+def _paged(name: str, x: torch.Tensor, k, v, layout: str, k_scale: float, v_scale: float):
+    """(packed description of the page pools, kv_heads, head_dim) for the C entry points; x holds the 16-bit values beside them."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor):
         raise RuntimeError(f"{name}: CUDA tensors are needed (this build has no CPU path)")
-    if x.dtype not in _DT or k.dtype != v.dtype or k.dtype not in (x.dtype, FP8):
+    dt, shape, stride, idx = k.dtype, k.shape, k.stride(), x.get_device()
+    if x.dtype not in _DT or v.dtype is not dt or (dt is not x.dtype and dt is not FP8):
         raise RuntimeError(f"{name}: fp16 or bf16 values, and page pools both of that type or both float8_e4m3fn")
-    if layout not in ("HND", "NHD") or k.dim() != 4 or v.shape != k.shape or v.stride() != k.stride() or k.stride(3) != 1 \
-            or k.device != x.device or v.device != x.device:
-        raise RuntimeError(f"{name}: page pools must be 4-D on the device of the values, with equal shapes and strides, "
-                           "layout HND or NHD")
-    if k.dtype != FP8 and (k_scale != 1.0 or v_scale != 1.0):
+    if len(shape) != 4 or v.shape != shape or v.stride() != stride or stride[3] != 1 or k.get_device() != idx or v.get_device() != idx:
+        raise RuntimeError(f"{name}: page pools must be 4-D on the device of the values, with equal shapes and strides")
+    if dt is not FP8 and (k_scale != 1.0 or v_scale != 1.0):
         raise RuntimeError(f"{name}: scales belong to float8_e4m3fn page pools")
-    shape, stride = k.shape, k.stride()
-    h, t = (1, 2) if layout == "HND" else (2, 1)
-    # a size-one dimension has no stride of its own
-    ts = stride[t] if shape[t] > 1 else (shape[3] if layout == "HND" else shape[2] * shape[3])
-    hs = stride[h] if shape[h] > 1 else (ts * shape[t] if layout == "HND" else shape[3])
-    ps = stride[0] if shape[0] > 1 else ts * shape[t] + hs * shape[h]
-    return Exl3PagedCache(k.data_ptr(), v.data_ptr(), ps, hs, ts, shape[0], shape[t], shape[h], shape[3],
-                          _KV_KIND[k.dtype], k_scale, v_scale)
+    page, heads, ps, hs, ts = _page_strides(shape, stride, layout)
+    return _PACK_CACHE(k.data_ptr(), v.data_ptr(), ps, hs, ts, shape[0], page, heads, shape[3], _KV_KIND[dt], k_scale, v_scale), heads, shape[3]
+
+
+def _page_strides(shape, stride, layout: str):
+    """(page size, heads, strides between pages, heads, tokens) of a pool; a size-one dimension has no stride of its own."""
+    if layout == "HND":
+        heads, page = shape[1], shape[2]
+        ts = stride[2] if page > 1 else shape[3]
+        hs = stride[1] if heads > 1 else ts * page
+    elif layout == "NHD":
+        page, heads = shape[1], shape[2]
+        ts = stride[1] if page > 1 else heads * shape[3]
+        hs = stride[2] if heads > 1 else shape[3]
+    else:
+        raise RuntimeError("layout must be HND or NHD")
+    return page, heads, stride[0] if shape[0] > 1 else ts * page + hs * heads, hs, ts
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, positions: torch.Tensor,
@@ -700,42 +716,41 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.
     pool (-1 for padding) is skipped.  A token whose position is outside the tables is left as it is.  positions and
     slots are int64 [T]; no two tokens may share a slot.  The queries go to q_out [T, q_heads, hd], or back to their
     place in qkv; returns them."""
-    cache = _paged("qk_norm_rope_append", qkv, k_pages, v_pages, layout, k_scale, v_scale)
-    dev, hd = qkv.device, cache.head_dim
-    _need(qkv.dim() == 2 and (qkv.stride(1) == 1) and q_heads > 0 and qkv.shape[1] >= (q_heads + 2 * cache.kv_heads) * hd,
+    cache, kvh, hd = _paged("qk_norm_rope_append", qkv, k_pages, v_pages, layout, k_scale, v_scale)
+    idx, dt = qkv.get_device(), qkv.dtype
+    _need(qkv.dim() == 2 and qkv.stride(1) == 1 and q_heads > 0 and qkv.shape[1] >= (q_heads + 2 * kvh) * hd,
           "qk_norm_rope_append: qkv must be [T, (q_heads + 2 kv_heads) * hd] with contiguous rows")
-    T = qkv.shape[0]
-    _ints(positions, "positions", dev, torch.int64)
-    _ints(slots, "slots", dev, torch.int64)
+    T, wide = qkv.shape
+    pos, slot = _ints(positions, "positions", idx, _I64), _ints(slots, "slots", idx, _I64)
     _need(positions.shape[0] == T and slots.shape[0] == T, "qk_norm_rope_append: positions and slots must be [T]")
-    rot, rows = 0, 1
-    _need((cos is None) == (sin is None), "qk_norm_rope_append: cos and sin belong together")
-    if cos is not None:
-        _cuda(cos, "cos", torch.float32)
-        _cuda(sin, "sin", torch.float32)
-        _need(cos.dim() == 2 and cos.shape == sin.shape and cos.device == dev and sin.device == dev,
-              "qk_norm_rope_append: cos and sin must be [max_pos, rot / 2] on the device of qkv")
-        rows, rot = cos.shape[0], 2 * cos.shape[1]
+    cp = sp = qw = kw = None
+    if cos is not None and sin is not None:
+        shape = cos.shape
+        for t in (cos, sin):
+            _need(isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.get_device() == idx and t.dim() == 2 and
+                  t.shape == shape and t.is_contiguous(),
+                  "qk_norm_rope_append: cos and sin must be fp32 [max_pos, rot / 2], contiguous, on the device of qkv")
+        rows, rot, cp, sp = shape[0], 2 * shape[1], cos.data_ptr(), sin.data_ptr()
     else:
-        rows = 2 ** 31 - 1                                # no table: no position is outside of it
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None:
-            _cuda(w, name, qkv.dtype)
-            _need(w.shape == (hd,) and w.device == dev, f"{name} must be [hd] on the device of qkv")
-    ldq = 0
+        _need(cos is None and sin is None, "qk_norm_rope_append: cos and sin belong together")
+        rows, rot = 2 ** 31 - 1, 0                        # no table: no position is outside of it
+    for w in (q_weight, k_weight):
+        _need(w is None or (isinstance(w, torch.Tensor) and w.dtype is dt and w.get_device() == idx and w.shape == (hd,) and
+                            w.is_contiguous()), "qk_norm_rope_append: the weights must be [hd] in the type of qkv, on its device")
+    if q_weight is not None:
+        qw = q_weight.data_ptr()
+    if k_weight is not None:
+        kw = k_weight.data_ptr()
+    ldq, qp = 0, None
     if q_out is not None:
-        _need(isinstance(q_out, torch.Tensor) and q_out.device == dev and q_out.dtype == qkv.dtype and
+        _need(isinstance(q_out, torch.Tensor) and q_out.get_device() == idx and q_out.dtype is dt and
               q_out.shape == (T, q_heads, hd) and q_out.stride(2) == 1 and (q_heads == 1 or q_out.stride(1) == hd),
               "qk_norm_rope_append: q_out must be [T, q_heads, hd] in the type of qkv, with contiguous heads")
-        ldq = q_out.stride(0) if T > 1 else q_heads * hd
-    if T == 0:
-        return q_out if q_out is not None else torch.as_strided(qkv, (0, q_heads, hd), (qkv.stride(0), hd, 1))
-    ld = qkv.stride(0) if T > 1 else -(-qkv.shape[1] // 8) * 8
-    _call(dev, lib().exl3_qk_norm_rope_append, qkv.data_ptr(), ld, None if q_out is None else q_out.data_ptr(), ldq,
-          None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-          0 if eps is None else 1, 0.0 if eps is None else eps, None if cos is None else cos.data_ptr(),
-          None if sin is None else sin.data_ptr(), rot, 1 if interleaved else 0, rows, positions.data_ptr(),
-          slots.data_ptr(), T, q_heads, 1 if qkv.dtype == torch.bfloat16 else 0, ctypes.byref(cache))
+        ldq, qp = q_out.stride(0) if T > 1 else q_heads * hd, q_out.data_ptr()
+    if T:
+        _call(idx, lib().exl3_qk_norm_rope_append, qkv.data_ptr(), qkv.stride(0) if T > 1 else -(-wide // 8) * 8, qp, ldq, qw, kw,
+              0 if eps is None else 1, 0.0 if eps is None else eps, cp, sp, rot, 1 if interleaved else 0, rows, pos, slot, T,
+              q_heads, 1 if dt is torch.bfloat16 else 0, cache)
     return q_out if q_out is not None else torch.as_strided(qkv, (T, q_heads, hd), (qkv.stride(0), hd, 1))
 
 
@@ -752,36 +767,33 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     that sees nothing gives zeros.  Page pools and block_table as for decode_attn_paged (q's type or float8_e4m3fn; page
     size a multiple of 16); tokens on a page number outside the pool are not visible.  Rows of q from starts[B] on are
     not read, those of `out` not written.  Returns [T, q_heads, hd] in q's type."""
-    cache = _paged("tree_attn_paged", q, k_pages, v_pages, layout, k_scale, v_scale)
-    dev, hd = q.device, cache.head_dim
+    cache, kvh, hd = _paged("tree_attn_paged", q, k_pages, v_pages, layout, k_scale, v_scale)
+    idx, dt = q.get_device(), q.dtype
     _need(q.dim() == 3 and q.shape[2] == hd and q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == hd),
           "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
-    T, qh = q.shape[0], q.shape[1]
-    _ints(block_table, "block_table", dev, torch.int32, 2)
-    _ints(seq_lens, "seq_lens", dev)
-    _ints(starts, "starts", dev)
-    B = block_table.shape[0]
+    T, qh, _ = q.shape
+    table, lens, first = _ints(block_table, "block_table", idx, _I32, 2), _ints(seq_lens, "seq_lens", idx), _ints(starts, "starts", idx)
+    B, width = block_table.shape
     _need(seq_lens.shape[0] == B and starts.shape[0] == B + 1, "tree_attn_paged: seq_lens must be [B], starts [B + 1]")
+    mask = None
     if tree_mask is not None:
-        _ints(tree_mask, "tree_mask", dev, torch.int64)
+        mask = _ints(tree_mask, "tree_mask", idx, _I64)
         _need(tree_mask.shape[0] == T, "tree_attn_paged: tree_mask must be [T]")
     if out is None:
-        out = torch.empty((T, qh, hd), dtype=q.dtype, device=dev)
+        out = torch.empty((T, qh, hd), dtype=dt, device=q.device)
     else:
-        _need(isinstance(out, torch.Tensor) and out.device == dev and out.dtype == q.dtype and out.shape == q.shape and
+        _need(isinstance(out, torch.Tensor) and out.get_device() == idx and out.dtype is dt and out.shape == q.shape and
               out.stride(2) == 1 and (qh == 1 or out.stride(1) == hd),
               "tree_attn_paged: out must be [T, heads, hd] in the type of q, with contiguous heads")
     if T == 0 or B == 0:
-        _need(1 <= max_drafts <= TREE_MAX_DRAFTS and qh > 0 and qh % cache.kv_heads == 0, "tree_attn_paged: bad max_drafts or heads")
+        _need(1 <= max_drafts <= TREE_MAX_DRAFTS and qh > 0 and qh % kvh == 0, "tree_attn_paged: bad max_drafts or heads")
         return out
     L, row = lib(), qh * hd
-    cref = ctypes.byref(cache)
-    need = L.exl3_tree_attn_workspace_bytes(B, qh, max_drafts, cref)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    _call(dev, L.exl3_tree_attn, q.data_ptr(), q.stride(0) if T > 1 else row, out.data_ptr(), out.stride(0) if T > 1 else row,
-          block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1], block_table.shape[1],
-          seq_lens.data_ptr(), starts.data_ptr(), None if tree_mask is None else tree_mask.data_ptr(), B, T, max_drafts, qh,
-          hd ** -0.5 if scale is None else scale, 1 if q.dtype == torch.bfloat16 else 0, cref,
+    need = L.exl3_tree_attn_workspace_bytes(B, qh, max_drafts, cache)
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+    _call(idx, L.exl3_tree_attn, q.data_ptr(), q.stride(0) if T > 1 else row, out.data_ptr(), out.stride(0) if T > 1 else row,
+          table, block_table.stride(0) if B > 1 else width, width, lens, first, mask, B, T, max_drafts, qh,
+          hd ** -0.5 if scale is None else scale, 1 if dt is torch.bfloat16 else 0, cache,
           None if ws is None else ws.data_ptr(), need)
     return out
 
@@ -806,46 +818,41 @@ def page_tables(max_seqs: int, pages_per_seq: int, num_pages: int, device) -> di
 
 
 def _tables(tables: dict, page_size: int):
+    """(device, number of pages, packed tables)."""
     bt, lens, held, refs, free, cnt = (tables[n] for n in ("block_table", "seq_lens", "held", "refs", "free_list", "counters"))
-    if not isinstance(bt, torch.Tensor) or bt.device.type != "cuda":
+    if not isinstance(bt, torch.Tensor) or not bt.is_cuda:
         raise RuntimeError("block_table must be a CUDA tensor (this build has no CPU path)")
-    dev = bt.device
-    _ints(bt, "block_table", dev, torch.int32, 2)
-    for t, name in ((lens, "seq_lens"), (held, "held"), (refs, "refs"), (free, "free_list"), (cnt, "counters")):
-        _ints(t, name, dev)
-    S, P, N = bt.shape[0], bt.shape[1], refs.shape[0]
-    _need(lens.shape[0] == S and held.shape[0] == S and free.shape[0] == N and cnt.shape[0] == 2,
-          "page tables: seq_lens and held must be [max_seqs], free_list [num_pages], counters [2]")
-    return dev, Exl3PageTables(bt.data_ptr(), lens.data_ptr(), held.data_ptr(), refs.data_ptr(), free.data_ptr(),
-                               cnt.data_ptr(), bt.stride(0) if S > 1 else P, P, S, N, page_size)
+    idx = bt.get_device()
+    p = (_ints(bt, "block_table", idx, _I32, 2), _ints(lens, "seq_lens", idx), _ints(held, "held", idx),
+         _ints(refs, "refs", idx), _ints(free, "free_list", idx), _ints(cnt, "counters", idx))
+    (S, P), N = bt.shape, refs.shape[0]
+    if lens.shape[0] != S or held.shape[0] != S or free.shape[0] != N or cnt.shape[0] != 2:
+        raise RuntimeError("page tables: seq_lens and held must be [max_seqs], free_list [num_pages], counters [2]")
+    return idx, N, _PACK_TABLES(*p, bt.stride(0) if S > 1 else P, P, S, N, page_size)
 
 
-def _pools(pools, layout: str, dev: torch.device, num_pages: int):
-    """The page pools of all layers: one tensor [n, pages, ...] or a sequence of equal pools."""
+def _pools(pools, layout: str, idx: int, num_pages: int):
+    """The page pools of all layers, packed (with what has to live as long): one tensor [n, pages, ...] or a sequence of
+    equal pools."""
     if isinstance(pools, torch.Tensor):
-        _need(pools.dim() == 5 and pools.device == dev, "pools must be [n, pages, ...] on the device of the tables, or a list of pools")
-        n, shape, stride = pools.shape[0], pools.shape[1:], pools.stride()[1:]
-        size = pools.element_size()
-        base, step = pools.data_ptr(), pools.stride(0) * size
-        where = [base + i * step for i in range(n)]
+        _need(pools.dim() == 5 and pools.get_device() == idx, "pools must be [n, pages, ...] on the device of the tables, or a list of pools")
+        shape, stride, size = pools.shape, pools.stride(), pools.element_size()
+        n, step, shape, stride = shape[0], stride[0] * size, shape[1:], stride[1:]
+        _need(n <= 1 or step > 0, "pools must be different pools")
+        where = ctypes.c_void_p(pools.data_ptr())
     else:
         n = len(pools)
-        _need(n > 0 and all(isinstance(p, torch.Tensor) and p.device == dev and p.dim() == 4 for p in pools),
+        _need(n > 0 and all(isinstance(p, torch.Tensor) and p.get_device() == idx and p.dim() == 4 for p in pools),
               "pools must be 4-D tensors on the device of the tables")
-        shape, stride, size = pools[0].shape, pools[0].stride(), pools[0].element_size()
-        _need(all(p.shape == shape and p.stride() == stride and p.dtype == pools[0].dtype for p in pools),
+        shape, stride, dt, size, step = pools[0].shape, pools[0].stride(), pools[0].dtype, pools[0].element_size(), 0
+        _need(all(p.shape == shape and p.stride() == stride and p.dtype is dt for p in pools),
               "pools must have equal shapes, strides and types")
-        where = [p.data_ptr() for p in pools]
-    _need(len(set(where)) == n, "pools must be different pools")
-    ptrs = (ctypes.c_void_p * max(n, 1))(*where)
-    _need(layout in ("HND", "NHD") and stride[3] == 1, "pools: layout HND or NHD, contiguous rows")
-    _need(shape[0] == num_pages, "pools must have as many pages as the tables count")
-    h, t = (1, 2) if layout == "HND" else (2, 1)
-    ts = stride[t] if shape[t] > 1 else (shape[3] if layout == "HND" else shape[2] * shape[3])
-    hs = stride[h] if shape[h] > 1 else (ts * shape[t] if layout == "HND" else shape[3])
-    ps = stride[0] if shape[0] > 1 else ts * shape[t] + hs * shape[h]
-    return shape[t], Exl3PagePools(ctypes.cast(ptrs, ctypes.POINTER(ctypes.c_void_p)), ps * size, hs * size, ts * size, n,
-                                   shape[h], shape[3] * size)
+        ptrs = [p.data_ptr() for p in pools]
+        _need(len(set(ptrs)) == n, "pools must be different pools")
+        where = (ctypes.c_void_p * n)(*ptrs)
+    _need(stride[3] == 1 and shape[0] == num_pages, "pools must have contiguous rows and as many pages as the tables count")
+    _, heads, ps, hs, ts = _page_strides(shape, stride, layout)
+    return where, _PACK_POOLS(ctypes.addressof(where), ps * size, hs * size, ts * size, n, heads, shape[3] * size, step)
 
 
 def _page_size(pools, layout: str) -> int:
@@ -858,19 +865,17 @@ def cache_fork(pools, tables: dict, parents: torch.Tensor, children: torch.Tenso
     """Make sequences children[i] (which hold nothing) copies of parents[i] (int32 [n], n <= 1024): full pages are
     shared, the used rows of a partial last page are copied to a new page in every pool.  pools: the K and V page
     pools of all layers, one tensor [n_pools, pages, ...] or a list of equal pools (at most 256); tables: page_tables()."""
-    dev, tab = _tables(tables, _page_size(pools, layout))
-    _, pl = _pools(pools, layout, dev, tab.num_pages)
-    _ints(parents, "parents", dev)
-    _ints(children, "children", dev)
+    idx, pages, tab = _tables(tables, _page_size(pools, layout))
+    keep, pl = _pools(pools, layout, idx, pages)
+    par, kid = _ints(parents, "parents", idx), _ints(children, "children", idx)
     n = parents.shape[0]
     _need(children.shape[0] == n, "cache_fork: as many children as parents")
     if n == 0:
         return
     L = lib()
     need = L.exl3_cache_fork_workspace_bytes(n)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    _call(dev, L.exl3_cache_fork, ctypes.byref(pl), ctypes.byref(tab), parents.data_ptr(), children.data_ptr(), n,
-          None if ws is None else ws.data_ptr(), need)
+    ws = torch.empty((need,), dtype=torch.uint8, device=parents.device) if need else None
+    _call(idx, L.exl3_cache_fork, pl, tab, par, kid, n, None if ws is None else ws.data_ptr(), need)
 
 
 def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_size: int, tokens: int):
@@ -879,16 +884,16 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     position, one sequence after the other, the sequences' first rows (what qk_norm_rope_append and tree_attn_paged
     take), and the lengths before.  Slots behind the last token, and those of a sequence that could not be served
     (counters[1]), are -1."""
-    dev, tab = _tables(tables, page_size)
-    _ints(seqs, "seqs", dev)
-    _ints(counts, "counts", dev)
+    idx, _, tab = _tables(tables, page_size)
+    seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
     n = seqs.shape[0]
     _need(counts.shape[0] == n and n > 0 and tokens >= 0, "cache_reserve: seqs and counts must be [n], n > 0")
-    where = torch.empty((2, tokens), dtype=torch.int64, device=dev)
-    rows = torch.empty((2 * n + 1,), dtype=torch.int32, device=dev)
-    slots, positions, starts, base = where[0], where[1], rows[:n + 1], rows[n + 1:]
-    _call(dev, lib().exl3_cache_reserve, ctypes.byref(tab), seqs.data_ptr(), counts.data_ptr(), n, slots.data_ptr(),
-          positions.data_ptr(), tokens, starts.data_ptr(), base.data_ptr())
+    where = torch.empty((2, tokens), dtype=_I64, device=seqs.device)
+    rows = torch.empty((2 * n + 1,), dtype=_I32, device=seqs.device)
+    slots, positions = where.unbind(0)
+    starts, base = rows.split((n + 1, n))
+    _call(idx, lib().exl3_cache_reserve, tab, seq, cnt, n, slots.data_ptr(), positions.data_ptr(), tokens, starts.data_ptr(),
+          base.data_ptr())
     return slots, positions, starts, base
 
 
@@ -897,24 +902,21 @@ def cache_accept(pools, tables: dict, seqs: torch.Tensor, base: torch.Tensor, dr
     """After drafts[i] drafted tokens behind base[i] of sequence seqs[i] were verified: move the rows of the accepted
     drafts path[i, :taken[i]] (int32 [n, most], most <= 64) to base[i], base[i] + 1, .. in every pool, and set seq_lens
     to base + taken.  Pages stay with the sequence.  pools, tables: as for cache_fork."""
-    dev, tab = _tables(tables, _page_size(pools, layout))
-    _, pl = _pools(pools, layout, dev, tab.num_pages)
-    for t, name in ((seqs, "seqs"), (base, "base"), (drafts, "drafts"), (taken, "taken")):
-        _ints(t, name, dev)
-    _ints(path, "path", dev, torch.int32, 2)
+    idx, pages, tab = _tables(tables, _page_size(pools, layout))
+    keep, pl = _pools(pools, layout, idx, pages)
+    p = (_ints(seqs, "seqs", idx), _ints(base, "base", idx), _ints(drafts, "drafts", idx), _ints(path, "path", idx, _I32, 2),
+         _ints(taken, "taken", idx))
     n, most = path.shape
     _need(seqs.shape[0] == n and base.shape[0] == n and drafts.shape[0] == n and taken.shape[0] == n,
           "cache_accept: seqs, base, drafts and taken must be [n], path [n, most]")
     if n == 0:
         return
-    _call(dev, lib().exl3_cache_accept, ctypes.byref(pl), ctypes.byref(tab), seqs.data_ptr(), base.data_ptr(),
-          drafts.data_ptr(), path.data_ptr(), path.stride(0) if n > 1 else most, most, taken.data_ptr(), n)
+    _call(idx, lib().exl3_cache_accept, pl, tab, p[0], p[1], p[2], p[3], path.stride(0) if n > 1 else most, most, p[4], n)
 
 
 def cache_free(tables: dict, seqs: torch.Tensor) -> None:
     """Give up the pages of the sequences seqs (int32 [n], n <= 1024); those that nobody holds any more are free again."""
-    dev, tab = _tables(tables, 1)
-    _ints(seqs, "seqs", dev)
-    if seqs.shape[0] == 0:
-        return
-    _call(dev, lib().exl3_cache_free, ctypes.byref(tab), seqs.data_ptr(), seqs.shape[0])
+    idx, _, tab = _tables(tables, 1)
+    seq = _ints(seqs, "seqs", idx)
+    if seqs.shape[0]:
+        _call(idx, lib().exl3_cache_free, tab, seq, seqs.shape[0])
