@@ -8,9 +8,10 @@
 // before the first is used.  What it takes to stay at that bound is few instructions per value: weight, cosine and sine
 // are multiplied once per token and kind of head (a = w_i c_i, b = +- w_partner s_i), a head then costs
 // r (x a + x_partner b) in packed fp32, the partner values come by shuffle in the input's 16-bit form, and four heads'
-// sums of squares are reduced together (ten shuffles instead of twenty).  Many tokens: one warp per token; few: up to
-// eight warps share a token's heads, since then latency counts.  Everything is computed in fp32 from the inputs and
-// rounded once, to fp16 / bf16 or straight to e4m3.
+// sums of squares are reduced together (ten shuffles instead of twenty), while the loads of the next four are in flight.
+// 16384 tokens of 24 / 4 heads of 256: 100 us, 5.5 TB/s, 85 % of the measured copy rate (one head after the other with
+// its weights read beside it: 163 us).  Few tokens take a CTA each instead of a warp, since then latency counts.
+// Everything is computed in fp32 from the inputs and rounded once, to fp16 / bf16 or straight to e4m3.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -38,12 +39,7 @@ struct AppendParams {
 };
 
 constexpr int kAppendWarps = 8;
-#ifndef APPEND_ROWS
-#define APPEND_ROWS 1536
-#endif
-#ifndef APPEND_OCC
-#define APPEND_OCC 3
-#endif
+constexpr int kFewTokens = 1024;
 
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4 &u, float2 (&f)[4]) {
@@ -212,7 +208,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_token_kernel(const _
 
 // Many tokens: a warp per token.
 template <typename T, bool FP8, int HD, bool ADJACENT>
-__global__ void __launch_bounds__(kAppendWarps * 32, APPEND_OCC) append_stream_kernel(const __grid_constant__ AppendParams P) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 3) append_stream_kernel(const __grid_constant__ AppendParams P) {
     constexpr int kLanes = HD / 8;            // lanes of a head
     constexpr int kPer = 32 / kLanes;         // heads of a warp
     constexpr int kFly = 4;                   // heads in flight per lane
@@ -339,8 +335,9 @@ __global__ void __launch_bounds__(kAppendWarps * 32, APPEND_OCC) append_stream_k
 
 template <typename T, bool FP8, int HD>
 static cudaError_t launch_append(const AppendParams &P, bool adjacent, cudaStream_t st) {
-    // A CTA per token up to 1536 tokens (10.3 against 11.0 us at 1024), a warp per token above (17.8 against 20 us at 2048).
-    if (P.tokens <= APPEND_ROWS) {
+    // Measured with 24 / 4 heads of 256 (us, a CTA per token against a warp per token): 4.2 / 10.4 at 5 tokens, 10.7 / 11.7 at
+    // 1024 into an e4m3 cache, 14.3 / 14.4 at 1024 and 24.6 / 20.6 at 2048 into an fp16 one, 163 / 100 at 16384.
+    if (P.tokens <= kFewTokens) {
         auto kernel = adjacent ? append_token_kernel<T, FP8, HD, true> : append_token_kernel<T, FP8, HD, false>;
         return launch_pdl(kernel, dim3(P.tokens), dim3(kAppendWarps * 32), 0, st, P);
     }
