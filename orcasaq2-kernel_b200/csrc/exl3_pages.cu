@@ -124,6 +124,27 @@ __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_co
     if (i == 0) T.counters[0] = left - min(total, left);
 }
 
+// Element e = (a, b, c) of an array [..][nb][nc], walked in steps of a fixed number of elements: two additions and carries
+// a step (divisions were most of the copying kernels' instructions).
+struct Walk3 {
+    int a, b, c, da, db, dc, nb, nc;
+    __device__ __forceinline__ Walk3(int e, int step, int nb_, int nc_) : nb(nb_), nc(nc_) {
+        split(e, a, b, c);
+        split(step, da, db, dc);
+    }
+    __device__ __forceinline__ void split(int e, int &x, int &y, int &z) const {
+        const int r = e / nc;
+        z = e - r * nc;
+        x = r / nb;
+        y = r - x * nb;
+    }
+    __device__ __forceinline__ void next() {
+        c += dc; b += db; a += da;
+        if (c >= nc) { c -= nc; ++b; }
+        if (b >= nb) { b -= nb; ++a; }
+    }
+};
+
 struct PoolList { void *pool[EXL3_PAGES_MAX_POOLS]; };
 struct RowGeom { long long page_stride, head_stride, tok_stride; int heads, row_bytes; };    // strides in bytes
 
@@ -154,20 +175,18 @@ __global__ void __launch_bounds__(kCopyThreads) fork_copy_kernel(const __grid_co
     const int chunks = G.row_bytes >> 4;                              // 16-byte pieces of a row
     const int work = G.heads * q.rest * chunks;
     constexpr int kFly = 4;                                           // loads in flight per thread
+    // rows in the order they lie in memory: by token when a token's heads are adjacent, else by head
+    const bool by_token = G.head_stride < G.tok_stride;
+    const long long outer = by_token ? G.tok_stride : G.head_stride, inner = by_token ? G.head_stride : G.tok_stride;
+    Walk3 w(threadIdx.x, kCopyThreads, by_token ? G.heads : q.rest, chunks);
     for (int e0 = threadIdx.x; e0 < work; e0 += kFly * kCopyThreads) {
         uint4 v[kFly];
         long long off[kFly];
 #pragma unroll
         for (int u = 0; u < kFly; ++u) {
-            const int e = e0 + u * kCopyThreads;
-            if (e < work) {
-                const int r = e / chunks, x = e - r * chunks;
-                // rows in the order they lie in memory: by token when a token's heads are adjacent, else by head
-                const int h = G.head_stride < G.tok_stride ? r % G.heads : r / q.rest;
-                const int tok = G.head_stride < G.tok_stride ? r / G.heads : r % q.rest;
-                off[u] = h * G.head_stride + tok * G.tok_stride + (x << 4);
-                v[u] = *reinterpret_cast<const uint4 *>(src + off[u]);
-            }
+            off[u] = w.a * outer + w.b * inner + (w.c << 4);
+            if (e0 + u * kCopyThreads < work) v[u] = *reinterpret_cast<const uint4 *>(src + off[u]);
+            w.next();
         }
 #pragma unroll
         for (int u = 0; u < kFly; ++u)
@@ -342,11 +361,13 @@ __global__ void __launch_bounds__(kBookThreads) free_kernel(const __grid_constan
 struct AcceptParams {
     Tables t;
     const int *seqs, *base, *drafts, *path, *taken;
-    int n, path_stride, most, heads;    // heads: of one CTA
+    int n, path_stride, most, heads, pools, per;    // heads, per (pools): of one CTA; pools: in all
 };
 
-// grid (n, pools, head groups): one CTA moves the accepted rows of one sequence in some heads of one pool, through
-// shared memory, so that a path in any order is moved as if all rows were read before the first is written.
+// grid (n, pool groups, head groups): one CTA moves the accepted rows of one sequence in some heads of some pools, through
+// shared memory, so that a path in any order is moved as if all rows were read before the first is written.  Finding the
+// rows is a chain of four dependent loads, so a CTA does it once for several pools, and reads the next pool's rows while
+// it writes one's (64 sequences in 64 layers: 30 us, 4.8 TB/s; a CTA per pool took 40 us).
 constexpr int kAcceptThreads = 128;
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams P,
                                                                 const __grid_constant__ PoolList L,
@@ -383,22 +404,36 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
     }
     if (tid == 0 && blockIdx.y == 0 && blockIdx.z == 0) T.seq_lens[s] = base + taken;
     const int h0 = blockIdx.z * P.heads, nh = min(P.heads, G.heads - h0);
-    char *const pool = static_cast<char *>(L.pool[blockIdx.y]) + h0 * G.head_stride;
-    const int chunks = G.row_bytes >> 4, per_tok = nh * chunks;
+    const int chunks = G.row_bytes >> 4, work = taken * nh * chunks;
+    const int p0 = blockIdx.y * P.per, p1 = min(P.pools, p0 + P.per);
     const uint32_t stage = static_cast<uint32_t>(__cvta_generic_to_shared(rows_s));
-    const int work = taken * per_tok;
-    for (int e = tid; e < work; e += kAcceptThreads) {
-        const int j = e / per_tok, r = e - j * per_tok, h = r / chunks, x = r - h * chunks;
-        if (from_s[j] >= 0)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + 16 * e),
-                         "l"(pool + from_s[j] + h * G.head_stride + 16 * x) : "memory");
-    }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    __syncthreads();
-    for (int e = tid; e < work; e += kAcceptThreads) {
-        const int j = e / per_tok, r = e - j * per_tok, h = r / chunks, x = r - h * chunks;
-        if (from_s[j] >= 0)
-            *reinterpret_cast<uint4 *>(pool + to_s[j] + h * G.head_stride + 16 * x) = *reinterpret_cast<const uint4 *>(rows_s + 16 * e);
+    const int buffer = P.most * P.heads * G.row_bytes;
+    const Walk3 w0(tid, kAcceptThreads, nh, chunks);
+    const auto read = [&](int p) {
+        const char *const pool = static_cast<const char *>(L.pool[p]) + h0 * G.head_stride;
+        Walk3 w = w0;
+        for (int e = tid; e < work; e += kAcceptThreads, w.next())
+            if (from_s[w.a] >= 0)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(stage + (p & 1) * buffer + 16 * e),
+                             "l"(pool + from_s[w.a] + w.b * G.head_stride + 16 * w.c) : "memory");
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    read(p0);
+    for (int p = p0; p < p1; ++p) {
+        if (p + 1 < p1) {
+            read(p + 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+        }
+        __syncthreads();
+        char *const pool = static_cast<char *>(L.pool[p]) + h0 * G.head_stride;
+        Walk3 w = w0;
+        for (int e = tid; e < work; e += kAcceptThreads, w.next())
+            if (from_s[w.a] >= 0)
+                *reinterpret_cast<uint4 *>(pool + to_s[w.a] + w.b * G.head_stride + 16 * w.c) =
+                    *reinterpret_cast<const uint4 *>(rows_s + (p & 1) * buffer + 16 * e);
+        // (a thread writes what it read itself, and reads into the other buffer next: no barrier)
     }
 }
 
@@ -511,16 +546,20 @@ extern "C" int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_t
     if (n == 0) return EXL3_OK;
     P.seqs = (const int *)seqs; P.base = (const int *)base; P.drafts = (const int *)drafts; P.path = (const int *)path;
     P.taken = (const int *)taken; P.n = n; P.path_stride = path_stride; P.most = most;
-    // heads per CTA: up to 16 KB of rows, which leaves room for many CTAs on an SM
+    // heads per CTA: up to 16 KB of rows, twice, which leaves room for seven CTAs on an SM; pools per CTA: two such rounds of CTAs
     const int per_head = most * G.row_bytes;
     P.heads = per_head ? (16 * 1024) / per_head : G.heads;
     if (P.heads < 1) P.heads = 1;
     if (P.heads > G.heads) P.heads = G.heads;
-    const int smem = P.heads * per_head;
+    const int smem = 2 * P.heads * per_head;
     if (smem > 48 * 1024 &&
         cudaFuncSetAttribute(accept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return EXL3_E_LAUNCH;
-    const dim3 grid(n, pools->num_pools, (G.heads + P.heads - 1) / P.heads);
+    const int groups = (G.heads + P.heads - 1) / P.heads;
+    P.pools = pools->num_pools;
+    P.per = (int)((long long)n * P.pools * groups / (2 * 7 * 148));
+    P.per = P.per < 1 ? 1 : P.per > 32 ? 32 : P.per;
+    const dim3 grid(n, (P.pools + P.per - 1) / P.per, groups);
     if (launch_pdl(accept_kernel, grid, dim3(kAcceptThreads), smem, (cudaStream_t)stream, P, L, G) != cudaSuccess)
         return EXL3_E_LAUNCH;
     return launch_status();
