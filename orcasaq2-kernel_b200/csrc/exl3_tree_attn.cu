@@ -79,11 +79,11 @@ struct Shared {
     // A stage has a barrier for K and one for V: each of the two threads that issue MMAs sees only the rounds that are
     // its own (with one barrier a thread could be a whole round behind another's, and parity would mislead it).
     uint64_t k_full[5], v_full[5], empty[5];
-    uint64_t s_full[2], p_ready[2], v_here[2], pv_done[2], q_full, q_empty, o_free, drain[2];
+    uint64_t s_full[3], p_ready[3], v_here[3], pv_done[3], q_full, q_empty, o_free, drain[2];
     uint32_t tmem_base;
     int nonfinite[2];                         // of the current segment and the one before, in turn
     float top[kM], sum[2][kM];                // of the rows; sums of the two groups
-    int part[kMaxTiles][20];                  // blocks per tile and warp
+    int part[kMaxTiles][17];                  // blocks per tile and warp
     int first_seq, first_off;
 };
 static_assert(sizeof(Shared) <= 3072, "shared state");
@@ -91,6 +91,7 @@ static_assert(sizeof(Shared) <= 3072, "shared state");
 template <bool FP8, int HD>
 struct Cfg {
     static constexpr int kHalves = HD / kDims;                       // stages of a K or V block
+    static constexpr int kBufs = (512 - HD) / kTok;                  // scores in tensor memory: 2 blocks beside 256 dimensions, 3 beside 128
     static constexpr int kQBytes = kM * HD * 2;
     static constexpr int kStages = FP8 ? 3 : 5;
     static constexpr int kRaw = FP8 ? kStages : 0;
@@ -280,7 +281,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
 
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.k_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.v_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.empty[i]), 1); }
-        for (int i = 0; i < 2; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 4); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
+        for (int i = 0; i < C::kBufs; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 4); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
         mbar_init(s32(&S.q_full), 32); mbar_init(s32(&S.q_empty), 1);
         mbar_init(s32(&S.o_free), 8); mbar_init(s32(&S.drain[0]), 1); mbar_init(s32(&S.drain[1]), 1);
         S.nonfinite[0] = S.nonfinite[1] = 0;
@@ -297,6 +298,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
 
     // ---- this CTA's piece of the line: a thread has a run of sequences
     constexpr int kWarps = kThreads / 32;
+    static_assert(kWarps <= 17, "S.part");
     const int run = (P.batch + kThreads - 1) / kThreads, b0 = tid * run, b1 = min(P.batch, b0 + run);
     Seq s0 = {};
     if (b0 < b1) s0 = seq_of(P, b0);
@@ -369,17 +371,25 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 uint32_t phases = 0;                           // of the stages' K barriers
                 int stage = 0, cnt = 0;
                 bool ok = true;
+                const auto here = [&](int st) {
+                    const bool is = mbar_wait(s32(&S.k_full[st]), phases >> st & 1, status);
+                    phases ^= 1u << st;
+                    return is;
+                };
                 while (ok && wk.next()) {
                     ok = mbar_wait(s32(&S.q_full), wk.index & 1, status);
                     if (!ok) break;
                     fence_async();                             // the copies were other warps', plain ones
                     for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
-                        if (cnt >= 2) ok = mbar_wait(s32(&S.pv_done[cnt & 1]), ((cnt - 2) >> 1) & 1, status);   // P(cnt - 2) was used
-                        const uint32_t d = tmem + HD + (cnt & 1) * kTok;
+                        const int buf = cnt % C::kBufs;
+                        const uint32_t phase = cnt / C::kBufs & 1;
+                        // (128 dimensions: K is mostly there, and P the last to come; 256: the first half need not wait for the second)
+                        if constexpr (H == 1) ok = here(stage);
+                        if (ok && cnt >= C::kBufs) ok = mbar_wait(s32(&S.pv_done[buf]), phase ^ 1u, status);    // the P that lay there was used
+                        const uint32_t d = tmem + HD + buf * kTok;
                         for (int h = 0; h < H && ok; ++h) {
-                            ok = mbar_wait(s32(&S.k_full[stage]), phases >> stage & 1, status);
+                            if constexpr (H > 1) ok = here(stage);
                             if (!ok) break;
-                            phases ^= 1u << stage;
                             if constexpr (!FP8) fence_async();
                             fence_after_sync();
                             const uint64_t kd = kdesc + (uint32_t)(stage * (kStageBytes >> 4)), qd = qdesc + (uint32_t)(h * (2 * kM * 128 >> 4));
@@ -389,7 +399,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                             umma_commit(s32(&S.empty[stage]));
                             if (++stage == C::kStages) stage = 0;
                         }
-                        umma_commit(s32(&S.s_full[cnt & 1]));
+                        umma_commit(s32(&S.s_full[buf]));
                         // over V(i - 1) to the next K; behind the last K lie V of the last two blocks
                         const int skip = i + 1 == wk.nb ? (wk.nb > 1 ? 2 * H : H) : i ? H : 0;
                         stage = (stage + skip) % C::kStages;
@@ -410,6 +420,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 bool ok = true;
                 while (ok && wk.next()) {
                     for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
+                        const int buf = cnt % C::kBufs;
                         // before V(i) lies K(i + 1), before V(0) also K(0)
                         stage = (stage + (i + 1 < wk.nb ? H : 0) + (i ? 0 : H)) % C::kStages;
                         int st = stage;
@@ -419,22 +430,22 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                             if (++st == C::kStages) st = 0;
                         }
                         if (!ok) break;
-                        mbar_arrive(s32(&S.v_here[cnt & 1]));
-                        ok = mbar_wait(s32(&S.p_ready[cnt & 1]), (cnt >> 1) & 1, status);
+                        mbar_arrive(s32(&S.v_here[buf]));
+                        ok = mbar_wait(s32(&S.p_ready[buf]), cnt / C::kBufs & 1, status);
                         if (ok && i == 0 && wk.index) ok = mbar_wait(s32(&S.o_free), (wk.index - 1) & 1, status);
                         if (!ok) break;
                         if constexpr (!FP8) fence_async();
                         fence_after_sync();
                         for (int h = 0; h < H; ++h) {
                             const uint64_t vd = vdesc + (uint32_t)(stage * (kStageBytes >> 4));
-                            const uint32_t p = tmem + HD + (cnt & 1) * kTok + h * 32;
+                            const uint32_t p = tmem + HD + buf * kTok + h * 32;
 #pragma unroll
                             for (int k = 0; k < kTok / H / 16; ++k)
                                 umma_f16_ts(tmem, p + k * 8, vd + (k * (HD * 32) >> 4), idesc, i || h || k);
                             umma_commit(s32(&S.empty[stage]));
                             if (++stage == C::kStages) stage = 0;
                         }
-                        umma_commit(s32(&S.pv_done[cnt & 1]));
+                        umma_commit(s32(&S.pv_done[buf]));
                     }
                 }
                 umma_commit(s32(&S.drain[1]));
@@ -500,7 +511,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     if (tok0 + kTok <= ctx) return;
                     const int from = max(0, ctx - tok0), upto = min(kTok, wk.s.len - tok0);
                     const int vpos = pos + H + 2 * H * i + (i + 1 < wk.nb ? H : 0);
-                    hold(&S.v_here[n & 1], (n >> 1) & 1);      // (announced by the MMA thread, which looks at every stage in its turn)
+                    hold(&S.v_here[n % C::kBufs], n / C::kBufs & 1);      // (announced by the MMA thread, which looks at every stage in its turn)
                     constexpr int kUnits = HD / 8, kRowsV = kTok / H;           // 16-byte units of a row, rows of a stage
                     for (int e = row; e < (upto - from) * kUnits; e += 128) {
                         const int r = from + e / kUnits, u = e % kUnits, st = (vpos + r / kRowsV) % C::kStages, q = r % kRowsV;
@@ -517,7 +528,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 const auto ready = [&](int n) {
                     fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(s32(&S.p_ready[n & 1]));
+                    if (lane == 0) mbar_arrive(s32(&S.p_ready[n % C::kBufs]));
                 };
                 for (int i = (cnt ^ side) & 1; i < wk.nb; i += 2) {
                     const int n = cnt + i, tok0 = (wk.blk + i) * kTok;         // n: number of the block in the CTA
@@ -540,31 +551,34 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     // caches, and the warps waited for instructions more often than for anything but loads.  Nor did it pay to take
                     // the exponentials against the maximum known so far and read the scores once: 85 against 79 us at 61 drafts over
                     // 32768 tokens, the probabilities being in registers until that maximum is confirmed, and the loop unrolled.)
-                    const uint32_t s_t = tmem + lane_base + HD + (n & 1) * kTok;
-                    const auto load = [&](int k, uint32_t (&y)[32]) {          // scores, minus infinity where nothing is seen
-                        tmem_ld32(s_t + 32 * k, y);
-                        const uint32_t vis = masked ? seen(k) : ~0u;
-                        tmem_wait_ld();
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) y[e] = vis >> e & 1 ? y[e] : 0xFF800000u;
-                        }
-                    };
-                    hold(&S.s_full[n & 1], (n >> 1) & 1);
+                    const uint32_t s_t = tmem + lane_base + HD + n % C::kBufs * kTok;
+                    hold(&S.s_full[n % C::kBufs], n / C::kBufs & 1);
                     if (32 * quarter >= rows) {                // no rows in this quarter: whatever lies there as P stays in its lanes
                         clean(n, i, tok0);
                         ready(n);
                         continue;
                     }
                     float mx = -INFINITY;
-#pragma unroll 1
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t y[32];
-                        load(k, y);
+                    const auto mask = [&](int k, uint32_t (&y)[32]) {          // minus infinity where nothing is seen
+                        if (masked) {
+                            const uint32_t vis = seen(k);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) y[e] = vis >> e & 1 ? y[e] : 0xFF800000u;
+                        }
+                    };
+                    const auto greatest = [&](int k, uint32_t (&y)[32]) {
+                        mask(k, y);
                         float m4[4] = {mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                         for (int e = 0; e < 32; ++e) m4[e & 3] = fmaxf(m4[e & 3], __uint_as_float(y[e]));
                         mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                    };
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t y[32];
+                        tmem_ld32(s_t + 32 * k, y);
+                        tmem_wait_ld();
+                        greatest(k, y);
                     }
                     mx = mx == -INFINITY ? mx : mx * P.scale_log2;
                     if (i > 0) {                               // the maximum as the block before left it, and this group's sum with it
@@ -576,9 +590,9 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     const bool raise = mx > top + kRaise || (top == -INFINITY && mx > top);
                     const float corr = raise ? ex2(top - mx) : 1.f;    // 0 when nothing was seen before
                     if (raise) { top = mx; sum2.x *= corr; sum2.y *= corr; }
-                    S.top[row] = top;
+                    if (raise || i == 0) S.top[row] = top;
                     if (__any_sync(0xffffffffu, raise) && i > 0) {
-                        hold(&S.pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+                        hold(&S.pv_done[(n - 1) % C::kBufs], (n - 1) / C::kBufs & 1);
 #pragma unroll 1
                         for (int c = 0; c < HD; c += 32) {
                             uint32_t o[32];
@@ -592,10 +606,9 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     if (i + 1 < wk.nb) pass_on(1 + 4 * side + quarter);
                     const float shift = top == -INFINITY ? 0.f : top;
                     const float2 mul = make_float2(P.scale_log2, P.scale_log2), sub = make_float2(-shift, -shift);
-#pragma unroll 1
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t y[32], p[16];
-                        load(k, y);
+                    const auto exps = [&](int k, uint32_t (&y)[32]) {
+                        uint32_t p[16];
+                        mask(k, y);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             float2 a = fma2(make_float2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1])), mul, sub);
@@ -605,6 +618,13 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                             p[e] = Type16<T>::pack(a.x, a.y);
                         }
                         tmem_st16(s_t + 16 * k, p);            // over scores that were read
+                    };
+#pragma unroll 1
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t y[32];
+                        tmem_ld32(s_t + 32 * k, y);
+                        tmem_wait_ld();
+                        exps(k, y);
                     }
                     clean(n, i, tok0);
                     tmem_wait_st();
@@ -614,7 +634,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 cnt += wk.nb;
                 softmax_sync();                                // S.top is the last block's now; and (for the group that had not the
                                                                // last block) its scores have been there, so all products but two
-                hold(&S.pv_done[(cnt - 1) & 1], ((cnt - 1) >> 1) & 1);
+                hold(&S.pv_done[(cnt - 1) % C::kBufs], (cnt - 1) / C::kBufs & 1);
                 {
                     const float before = top;
                     top = S.top[row];
