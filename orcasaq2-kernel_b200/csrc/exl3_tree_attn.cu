@@ -27,9 +27,10 @@
 // filled with zeros instead of read, and non-finite V values of drafts, which some rows see and others do not, are
 // zeroed before the product and added to the rows that see them at the end (a path that finite caches never take).
 //
-// e4m3 caches: a pair of warps per stage fetches a raw stage of 16 KB beside it, every thread its own pieces (so it waits for nobody
-// else's), and widen them exactly to the 16-bit type of q into the swizzled stages, refilling the raw stage piece by
-// piece as they go; the scales fold into the softmax scale and the normalisation.
+// e4m3 caches: a pair of warps per stage fetches the 16 KB of rows into the stage's upper half and widens them in place,
+// from the front, exactly to the 16-bit type of q in the swizzled places; the scales fold into the softmax scale and the
+// normalisation.  (One warp alone needs ten cycles for a conversion of two values that four warps of a scheduler finish
+// in two.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -50,7 +51,6 @@ constexpr int kM = 128;                       // rows of a tile
 constexpr int kTok = 128;                     // tokens of a block
 constexpr int kDims = 128;                    // dimensions of a stage
 constexpr int kStageBytes = kTok * kDims * 2; // 32 KB
-constexpr int kRawBytes = kTok * kDims;       // 16 KB of e4m3
 constexpr int kMaxTiles = 16;
 constexpr int kMaxGrid = 148;
 constexpr float kRaise = 8.f;                 // log2 units the maximum may lag behind
@@ -79,11 +79,14 @@ struct Shared {
     // A stage has a barrier for K and one for V: each of the two threads that issue MMAs sees only the rounds that are
     // its own (with one barrier a thread could be a whole round behind another's, and parity would mislead it).
     uint64_t k_full[5], v_full[5], empty[5];
-    uint64_t s_full[3], p_ready[3], v_here[3], pv_done[3], q_full, q_empty, o_free, drain[2];
+    uint64_t s_full[3], p_ready[3], v_here[3], pv_done[3], q_empty, o_free, drain[2];
     uint32_t tmem_base;
     int nonfinite[2];                         // of the current segment and the one before, in turn
-    float top[kM], sum[2][kM];                // of the rows; sums of the two groups
-    int part[kMaxTiles][17];                  // blocks per tile and warp
+    float top[kM];                            // of the rows
+    union {
+        int part[kMaxTiles][20];              // blocks per tile and warp (before the roles part)
+        float sum[2][kM];                     // sums of the two groups
+    };
     int first_seq, first_off;
 };
 static_assert(sizeof(Shared) <= 3072, "shared state");
@@ -93,10 +96,9 @@ struct Cfg {
     static constexpr int kHalves = HD / kDims;                       // stages of a K or V block
     static constexpr int kBufs = (512 - HD) / kTok;                  // scores in tensor memory: 2 blocks beside 256 dimensions, 3 beside 128
     static constexpr int kQBytes = kM * HD * 2;
-    static constexpr int kStages = FP8 ? 3 : 5;
-    static constexpr int kRaw = FP8 ? kStages : 0;
-    static constexpr int kThreads = 32 * (11 + (FP8 ? 2 : 1) * kStages);     // 2 MMA + 1 query + 8 softmax warps, one or two per stage
-    static constexpr int kSmem = kQBytes + kStages * kStageBytes + kRaw * kRawBytes + sizeof(Shared);
+    static constexpr int kStages = 5;
+    static constexpr int kThreads = 32 * (10 + (FP8 ? 2 : 1) * kStages);     // 2 MMA + 8 softmax warps, one or two per stage
+    static constexpr int kSmem = kQBytes + kStages * kStageBytes + sizeof(Shared);
 };
 
 
@@ -270,8 +272,8 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     constexpr int H = C::kHalves;
     constexpr int kThreads = C::kThreads;
     extern __shared__ __align__(1024) unsigned char smem[];      // (swizzle atoms are 1 KB)
-    unsigned char *const smQ = smem, *const ring = smQ + C::kQBytes, *const rawring = ring + C::kStages * kStageBytes;
-    Shared &S = *reinterpret_cast<Shared *>(rawring + C::kRaw * kRawBytes);
+    unsigned char *const smQ = smem, *const ring = smQ + C::kQBytes;
+    Shared &S = *reinterpret_cast<Shared *>(ring + C::kStages * kStageBytes);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned *const status = &g_tree_status;
     if (s32(smem) & 1023u) {
@@ -282,7 +284,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     if (tid == 0) {
         for (int i = 0; i < C::kStages; ++i) { mbar_init(s32(&S.k_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.v_full[i]), FP8 ? 2 : 32); mbar_init(s32(&S.empty[i]), 1); }
         for (int i = 0; i < C::kBufs; ++i) { mbar_init(s32(&S.s_full[i]), 1); mbar_init(s32(&S.p_ready[i]), 4); mbar_init(s32(&S.v_here[i]), 1); mbar_init(s32(&S.pv_done[i]), 1); }
-        mbar_init(s32(&S.q_full), 32); mbar_init(s32(&S.q_empty), 1);
+        mbar_init(s32(&S.q_empty), 1);
         mbar_init(s32(&S.o_free), 8); mbar_init(s32(&S.drain[0]), 1); mbar_init(s32(&S.drain[1]), 1);
         S.nonfinite[0] = S.nonfinite[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -298,7 +300,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
 
     // ---- this CTA's piece of the line: a thread has a run of sequences
     constexpr int kWarps = kThreads / 32;
-    static_assert(kWarps <= 17, "S.part");
+    static_assert(kWarps <= 20, "S.part");
     const int run = (P.batch + kThreads - 1) / kThreads, b0 = tid * run, b1 = min(P.batch, b0 + run);
     Seq s0 = {};
     if (b0 < b1) s0 = seq_of(P, b0);
@@ -361,25 +363,46 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     if (u1 > u0) {
         Walk wk(P, m, S.first_seq, S.first_off, u1 - u0);
         if (warp == 1) {
-            // ---------------- S = Q K^T.  Two threads issue the MMAs, one for each product: a thread's waits, fences and
-            // commits cost it about as much as the tensor cores need for its share of a block (one thread for both: 5050
-            // cycles a block, of which the tensor cores worked 2300)
-            if (lane == 0) {
-                constexpr uint32_t kType = __is_same(T, __half) ? 0u : (1u << 7 | 1u << 10);
-                const uint32_t idesc = umma_idesc_f16(kM, kTok) | kType | (P.negate ? 1u << 13 : 0u);      // bit 13: -A
-                const uint64_t qdesc = desc_sw128(s32(smQ), 16, 1024), kdesc = desc_sw128(s32(ring), 16, 2048);
-                uint32_t phases = 0;                           // of the stages' K barriers
-                int stage = 0, cnt = 0;
-                bool ok = true;
-                const auto here = [&](int st) {
-                    const bool is = mbar_wait(s32(&S.k_full[st]), phases >> st & 1, status);
-                    phases ^= 1u << st;
-                    return is;
-                };
-                while (ok && wk.next()) {
-                    ok = mbar_wait(s32(&S.q_full), wk.index & 1, status);
-                    if (!ok) break;
-                    fence_async();                             // the copies were other warps', plain ones
+            // ---------------- Q into shared memory, then S = Q K^T.  Two threads issue the MMAs, one for each product: a thread's
+            // waits, fences and commits cost it about as much as the tensor cores need for its share of a block (one thread for
+            // both: 5050 cycles a block, of which the tensor cores worked 2300)
+            constexpr uint32_t kType = __is_same(T, __half) ? 0u : (1u << 7 | 1u << 10);
+            const uint32_t idesc = umma_idesc_f16(kM, kTok) | kType | (P.negate ? 1u << 13 : 0u);      // bit 13: -A
+            const uint64_t qdesc = desc_sw128(s32(smQ), 16, 1024), kdesc = desc_sw128(s32(ring), 16, 2048);
+            constexpr int kUnits = HD / 8, kRows = 32 / kUnits;   // 16-byte units of a row of Q, rows of an instruction
+            const int u = lane % kUnits, sub = lane / kUnits;
+            int written = kM;                                  // rows of Q that may hold something
+            uint32_t phases = 0;                               // of the stages' K barriers
+            int stage = 0, cnt = 0;
+            bool ok = true;
+            const auto here = [&](int st) {
+                const bool is = mbar_wait(s32(&S.k_full[st]), phases >> st & 1, status);
+                phases ^= 1u << st;
+                return is;
+            };
+            while (ok && wk.next()) {
+                // rows (swizzled, K-major); those behind the last one are zero
+                if (wk.index) ok = __all_sync(0xffffffffu, mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status));
+                if (!ok) break;
+                const int rows = wk.rows(), upto = max(written, rows);
+                int r = sub, i = (kM * m + r) / P.G, g = kM * m + r - i * P.G;
+                const T *src = static_cast<const T *>(P.q) + (size_t)(wk.s.first + i) * P.q_stride + (size_t)(wk.hk * P.G + g) * HD + 8 * u;
+                const int di = kRows / P.G, dg = kRows - di * P.G;
+                const long long step = di * P.q_stride + dg * HD, wrap = P.q_stride - (long long)P.G * HD;
+                const uint32_t dst = s32(smQ) + (u >> 3) * (kM * 128);
+#pragma unroll 4
+                for (; r < rows; r += kRows) {
+                    copy16(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4), src);
+                    src += step; g += dg;
+                    if (g >= P.G) { g -= P.G; src += wrap; }
+                }
+                for (; r < upto; r += kRows)
+                    *reinterpret_cast<uint4 *>(smQ + (u >> 3) * (kM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+                written = rows;
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_async();
+                __syncwarp();
+                if (lane == 0) {
                     for (int i = 0; i < wk.nb && ok; ++i, ++cnt) {
                         const int buf = cnt % C::kBufs;
                         const uint32_t phase = cnt / C::kBufs & 1;
@@ -390,7 +413,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         for (int h = 0; h < H && ok; ++h) {
                             if constexpr (H > 1) ok = here(stage);
                             if (!ok) break;
-                            if constexpr (!FP8) fence_async();
+                            if constexpr (!FP8) fence_async();     // the copies were other warps', plain ones
                             fence_after_sync();
                             const uint64_t kd = kdesc + (uint32_t)(stage * (kStageBytes >> 4)), qd = qdesc + (uint32_t)(h * (2 * kM * 128 >> 4));
 #pragma unroll
@@ -406,6 +429,9 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     }
                     umma_commit(s32(&S.q_empty));
                 }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+            if (lane == 0) {
                 umma_commit(s32(&S.drain[0]));
                 mbar_wait(s32(&S.drain[0]), 0, status);
             }
@@ -451,41 +477,9 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 umma_commit(s32(&S.drain[1]));
                 mbar_wait(s32(&S.drain[1]), 0, status);
             }
-        } else if (warp == 2) {
-            // ---------------- query rows into shared memory (swizzled, K-major), rows behind the last one zero
-            constexpr int kUnits = HD / 8, kRows = 32 / kUnits;   // 16-byte units of a row, rows of an instruction
-            bool ok = true;
-            const int u = lane % kUnits, sub = lane / kUnits;
-            int filled = kM;                                   // rows that may hold something
-            while (ok && wk.next()) {
-                if (wk.index) {
-                    ok = mbar_wait(s32(&S.q_empty), (wk.index - 1) & 1, status, 200);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                }
-                const int rows = wk.rows(), upto = max(filled, rows);
-                constexpr int kStep = kRows;
-                int r = sub, i = (kM * m + r) / P.G, g = kM * m + r - i * P.G;
-                const T *src = static_cast<const T *>(P.q) + (size_t)(wk.s.first + i) * P.q_stride + (size_t)(wk.hk * P.G + g) * HD + 8 * u;
-                const int di = kStep / P.G, dg = kStep - di * P.G;
-                const long long step = di * P.q_stride + dg * HD, wrap = P.q_stride - (long long)P.G * HD;
-                const uint32_t dst = s32(smQ) + (u >> 3) * (kM * 128);
-#pragma unroll 4
-                for (; r < rows; r += kStep) {
-                    copy16(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4), src);
-                    src += step; g += dg;
-                    if (g >= P.G) { g -= P.G; src += wrap; }
-                }
-                for (; r < upto; r += kStep)
-                    *reinterpret_cast<uint4 *>(smQ + (u >> 3) * (kM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = make_uint4(0, 0, 0, 0);
-                fence_async();
-                filled = rows;
-                arrive_behind_copies(s32(&S.q_full));
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-        } else if (warp < 11) {
+        } else if (warp < 10) {
             // ---------------- softmax: thread = row = TMEM lane; group `side` takes the blocks of its parity
-            const int quarter = warp & 3, row = 32 * quarter + lane, side = (warp - 3) >> 2;
+            const int quarter = warp & 3, row = 32 * quarter + lane, side = (warp - 2) >> 2;
             const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
             constexpr int kCols = HD / 2;                      // of the result, this thread's half
             const uint32_t o_t = tmem + lane_base + side * kCols;
@@ -644,7 +638,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                 softmax_sync();
                 const float sum = S.sum[0][row] + S.sum[1][row];
                 const bool mend = S.nonfinite[wk.index & 1] != 0;       // uniform: all have written it before the barrier
-                if (tid == 96) S.nonfinite[wk.index & 1 ^ 1] = 0;      // read before the last barrier, written behind the next
+                if (tid == 64) S.nonfinite[wk.index & 1 ^ 1] = 0;      // read before the last barrier, written behind the next
                 const bool whole = wk.whole();
                 const float inv = sum == 0.f ? 0.f : P.v_scale / sum;
                 const int slot = 2 * blockIdx.x + (wk.index ? 1 : 0);
@@ -712,7 +706,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     }
                     __syncwarp();
                 }
-                if (!whole && wk.blk == 0 && tid == 96) {          // more parts follow in the next CTAs
+                if (!whole && wk.blk == 0 && tid == 64) {          // more parts follow in the next CTAs
                     const int q = U / W, r = U - q * W, last = u1 + wk.nblk - wk.nb - 1;     // the pair's last block
                     const int owner = last < r * (q + 1) ? last / (q + 1) : r + (last - r * (q + 1)) / q;
                     P.joins[blockIdx.x] = make_int4(wk.b, wk.hk, owner - w + 1, 2 * m + (wk.index ? 1 : 0));
@@ -729,7 +723,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
         } else if constexpr (!FP8) {
             // ---------------- cache rows into the ring: warp f fills stage f (one warp waits for all of a stage's releases: with
             // stages passed round it could be a whole round ahead of the others, and parity would mislead it)
-            const int f = warp - 11;
+            const int f = warp - 10;
             int filled = 0;
             bool ok = true;
             // wide stages (K, and V of 128 dimensions): an instruction is two rows of 256 bytes; tall ones: one of 512
@@ -806,95 +800,99 @@ tree_attn_kernel(const __grid_constant__ Params P) {
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
         } else {
-            // ---------------- e4m3 rows: warps 2 f and 2 f + 1 fill stage f by way of raw stage f (8 KB each), in instructions of
-            // four rows of 128 bytes, or two of 256
-            const int f = (warp - 11) >> 1, part = (warp - 11) & 1;
-            const uint32_t raw = s32(rawring) + f * kRawBytes + part * 8192 + 16 * lane;
-            const unsigned char *const rawp = rawring + f * kRawBytes + part * 8192 + 16 * lane;
-            bool ok = true;
+            // ---------------- e4m3 rows: warps 2 f and 2 f + 1 fill stage f, in eight quads of four instructions (two each): wide,
+            // sixteen tokens of 128 bytes, four to an instruction; tall, eight tokens of 256 bytes, two to an instruction.  Quad b
+            // arrives at 16 KB + 2 KB * b and becomes the 4 KB at 4 KB * b.
+            const int f = (warp - 10) >> 1, part = (warp - 10) & 1;
             int filled = 0;
-            // rows and pieces of a wide instruction (four rows of eight pieces) and a tall one (two of sixteen); a piece is two
-            // units of the swizzled row, and the lanes of a row start with different ones: no bank conflicts
+            bool ok = true;
+            // a lane's sixteen bytes are two units of the swizzled row, and the lanes of a row start with different ones: no bank
+            // conflicts
             const int wsub = lane >> 3, wu = lane & 7, tsub = lane >> 4, tu = lane & 15;
             const bool swap = lane & 4;
-            uint32_t wide_at[2], tall_at[4];                   // rows 4 j + wsub, 2 j + tsub of an atom
+            uint32_t wide_at[2], tall_at[2];                   // rows 4 j + wsub, 4 part + 2 j + tsub of an atom
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int r = 4 * j + wsub;
                 wide_at[j] = (wu >> 2) * 1024 + r * 128 + ((((wu & 3) * 2 + (swap ? 1 : 0)) ^ r) << 4);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 2 * j + tsub;
+            for (int j = 0; j < 2; ++j) {
+                const int r = 4 * part + 2 * j + tsub;
                 tall_at[j] = (tu >> 2) * 1024 + r * 128 + ((((tu & 3) * 2 + (swap ? 1 : 0)) ^ r) << 4);
             }
-            // fetch quarter b of this warp's part of a stage (sixteen tokens wide, or eight tall): four instructions
-            const auto fetch = [&](const Fill &fl, long long off, int rows, int b) {
+            const uint32_t raw = s32(ring) + f * kStageBytes + 16384 + part * 1024 + 16 * lane;
+            const auto fetch = [&](const Fill &fl, long long off, int rows) {
                 const unsigned char *const pool = static_cast<const unsigned char *>(fl.is_v ? P.v : P.k);
                 const bool tall = H == 2 && fl.is_v;
-                const int lane_of = tall ? 4 * fl.half + 2 * part + (b >> 1) : 4 * part + b;    // whose page it is
-                const int row0 = tall ? (b & 1) * 8 + tsub : wsub, inc = tall ? 2 : 4;
-                const unsigned char *src = pool + __shfl_sync(0xffffffffu, off, lane_of) + row0 * P.tok_stride + (tall ? 16 * tu : fl.half * kDims + 16 * wu);
-                const int n = __shfl_sync(0xffffffffu, rows, lane_of) - row0;
-                const long long step = inc * P.tok_stride;
+                const int inc = tall ? 2 : 4;
+                const long long step = inc * P.tok_stride, column = tall ? 16 * tu : fl.half * kDims + 16 * wu;
+#pragma unroll 1
+                for (int b = 0; b < 8; ++b) {
+                    const int lane_of = tall ? 4 * fl.half + (b >> 1) : b, row0 = tall ? (b & 1) * 8 + 4 * part + tsub : 8 * part + wsub;      // whose page it is
+                    const unsigned char *src = pool + __shfl_sync(0xffffffffu, off, lane_of) + row0 * P.tok_stride + column;
+                    const int n = __shfl_sync(0xffffffffu, rows, lane_of) - row0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i, src += step) {
-                    const bool real = inc * i < n;
-                    copy16(raw + b * 2048 + i * 512, real ? src : pool, real);
+                    for (int i = 0; i < 2; ++i, src += step) copy16(raw + b * 2048 + i * 512, inc * i < n ? src : pool, inc * i < n);
                 }
             };
             int skip = 0;
-            while (ok && wk.next()) {
+            while (wk.next()) {
                 const int fills = 2 * H * wk.nb;
                 int j = (f + C::kStages - skip) % C::kStages;
                 skip = (skip + fills) % C::kStages;
                 if (j >= fills) continue;
                 const long long head = wk.hk * P.head_stride;
                 Fill fl = fill_of<H>(j, wk.nb);
-                int t, at, page, rows = 0;
-                long long off = 0;
-                const auto look = [&]() {                      // lanes 0..7: the page of sixteen tokens each
-                    t = (wk.blk + fl.block) * kTok + 16 * (lane & 7);
-                    page = page_of(P, wk.b, t, wk.s.len, at);
-                };
-                const auto place = [&]() {
-                    const bool there = (unsigned)page < (unsigned)P.num_pages;
-                    off = there ? page * P.page_stride + head + at * P.tok_stride : 0ll;
-                    rows = there ? wk.s.len - t : 0;
-                };
-                look();
-                place();
-#pragma unroll 1
-                for (int b = 0; b < 4; ++b) fetch(fl, off, rows, b);
+                int t = (wk.blk + fl.block) * kTok + 16 * (lane & 7), at;      // lanes 0..7: sixteen tokens each
+                int page = page_of(P, wk.b, t, wk.s.len, at);
                 for (;;) {
+                    const bool there = (unsigned)page < (unsigned)P.num_pages;
+                    const long long off = there ? page * P.page_stride + head + at * P.tok_stride : 0ll;
+                    const int rows = there ? wk.s.len - t : 0;
                     const Fill now = fl;
                     const bool more = j + C::kStages < fills;
-                    if (more) { fl = fill_of<H>(j + C::kStages, wk.nb); look(); }
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    if (filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status, 40);
+                    if (more) {                                // the pages of the warp's next stage
+                        fl = fill_of<H>(j + C::kStages, wk.nb);
+                        t = (wk.blk + fl.block) * kTok + 16 * (lane & 7);
+                        page = page_of(P, wk.b, t, wk.s.len, at);
+                    }
+                    // (the pair meets at a barrier: after a wait that ran out it walks on without waiting, as the softmax warps do)
+                    if (ok && filled) ok = mbar_wait(s32(&S.empty[f]), (filled - 1) & 1, status, 40);
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    if (more) place();
-                    unsigned char *const dst = ring + f * kStageBytes + part * 16384;
+                    fetch(now, off, rows);
+                    asm volatile("cp.async.wait_all;" ::: "memory");
                     const bool tall = H == 2 && now.is_v;
+                    const unsigned char *src = ring + f * kStageBytes + 16384 + part * 1024 + 16 * lane;
+                    unsigned char *dst = ring + f * kStageBytes;
+                    // wide: rows 16 b + 8 part + 4 i + wsub; tall: 8 b + 4 part + 2 i + tsub
+                    const uint32_t at0 = tall ? tall_at[0] : wide_at[0] + part * 2048, at1 = tall ? tall_at[1] : wide_at[1] + part * 2048;
+                    const auto write = [&](const uint4 &v, uint32_t to) {
+                        uint4 one, two;
+                        widen4<T>(swap ? v.z : v.x, one.x, one.y);
+                        widen4<T>(swap ? v.w : v.y, one.z, one.w);
+                        widen4<T>(swap ? v.x : v.z, two.x, two.y);
+                        widen4<T>(swap ? v.y : v.w, two.z, two.w);
+                        *reinterpret_cast<uint4 *>(dst + to) = one;
+                        *reinterpret_cast<uint4 *>(dst + (to ^ 16)) = two;
+                    };
+                    // the first four quads become the lower half, which holds nothing; then both warps read the others and, when both
+                    // have, write them over the upper half
 #pragma unroll 1
-                    for (int b = 0; b < 4; ++b) {
+                    for (int b = 0; b < 4; b += 2) {
                         uint4 x[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4 *>(rawp + b * 2048 + i * 512);
+                        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + (b + (i >> 1)) * 2048 + (i & 1) * 512);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 lo, hi;
-                            widen4<T>(x[i].x, lo.x, lo.y);
-                            widen4<T>(x[i].y, lo.z, lo.w);
-                            widen4<T>(x[i].z, hi.x, hi.y);
-                            widen4<T>(x[i].w, hi.z, hi.w);
-                            // wide: rows 16 b + 4 i + wsub of 64; tall: 8 b + 2 i + tsub of 32
-                            const uint32_t to = tall ? tall_at[i] + b * 4096 : wide_at[i & 1] + b * 4096 + (i >> 1) * 2048;
-                            *reinterpret_cast<uint4 *>(dst + to) = swap ? hi : lo;
-                            *reinterpret_cast<uint4 *>(dst + (to ^ 16)) = swap ? lo : hi;
-                        }
-                        if (more) fetch(fl, off, rows, b);     // these pieces of the raw stage are in registers, and done with
+                        for (int i = 0; i < 4; ++i) write(x[i], (b + (i >> 1)) * 4096 + (i & 1 ? at1 : at0));
+                    }
+                    {
+                        uint4 x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + (4 + (i >> 1)) * 2048 + (i & 1) * 512);
+                        asm volatile("bar.sync %0, 64;" ::"r"(10 + f) : "memory");
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) write(x[i], (4 + (i >> 1)) * 4096 + (i & 1 ? at1 : at0));
                     }
                     fence_async();
                     __syncwarp();
@@ -904,7 +902,6 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     if (!more) break;
                 }
             }
-            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     }
     fence_before_sync();
