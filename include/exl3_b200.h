@@ -395,7 +395,7 @@ int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out, long long
  *                not read
  *   seq_lens     int32 [batch], drafts included; starts int32 [batch + 1], ascending; mask int64 [tokens] or NULL
  *   max_drafts   1 .. EXL3_TREE_MAX_DRAFTS, the largest number of drafts of a sequence; rows of a sequence from
- *                max_drafts on are not computed
+ *                max_drafts on are not computed; scale: finite
  *   cache        page_size a multiple of 16; q_heads a multiple of its kv_heads, at most 32 times as many
  *   workspace    exl3_tree_attn_workspace_bytes(...) bytes, 16-byte aligned, need not be cleared; calls that share it
  *                must not overlap on the device
@@ -456,15 +456,16 @@ int exl3_cache_fork(const exl3_page_pools *pools, const exl3_page_tables *tables
  * starts int32 [n + 1] (prefix sums of counts), and for the tokens, one sequence after the other, slots and positions
  * int64 [tokens] (what exl3_qk_norm_rope_append takes).  Tokens of a sequence that is not served, and entries behind
  * the last token, have slot -1 (the latter position 0).  tokens: room in the outputs, at most 2^20; a sequence that
- * does not fit is not served.  n >= 1.
+ * does not fit is not served, nor is one whose tokens would lie on a page that another sequence holds too (cut back by
+ * exl3_cache_accept into pages that it shares).  n >= 1.
  */
 int exl3_cache_reserve(const exl3_page_tables *tables, const void *seqs, const void *counts, int n, void *slots,
                        void *positions, int tokens, void *starts, void *base, void *stream);
 /*
  * After a tree of drafts[i] tokens behind base[i] was verified: the rows at base + path[i][j], j < taken[i] (at most
- * `most`, path is int32 [n][path_stride]), move to base + j in all pools, and seq_lens[seqs[i]] = base + taken.  The
- * pages stay with the sequence.  The rows are moved as if all were read before the first is written; pages that are
- * written must not be shared.
+ * `most`, path is int32 [n][path_stride], NULL when most is 0), move to base + j in all pools, and seq_lens[seqs[i]] =
+ * base + taken.  The pages stay with the sequence.  The rows are moved as if all were read before the first is written;
+ * pages that are written must not be shared.
  */
 int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_tables *tables, const void *seqs, const void *base,
                       const void *drafts, const void *path, int path_stride, int most, const void *taken, int n,

@@ -113,10 +113,8 @@ __global__ void __launch_bounds__(kBookThreads) fork_plan_kernel(const __grid_co
         if (served) {
             T.seq_lens[c] = len;
             T.held[c] = full + need;
-            if (dst >= 0) {
-                T.block_table[(size_t)c * T.bt_stride + full] = dst;
-                T.refs[dst] = 1;
-            }
+            if (need) T.block_table[(size_t)c * T.bt_stride + full] = dst;     // -1 from a broken stack or table: on no page
+            if (dst >= 0) T.refs[dst] = 1;
         } else {
             atomicOr(T.counters + 1, ok ? EXL3_PAGES_EXHAUSTED : EXL3_PAGES_BAD);
         }
@@ -227,6 +225,11 @@ __global__ void __launch_bounds__(kBookThreads) reserve_kernel(const __grid_cons
         held = T.held[s];
         const long long pages = ((long long)len + cnt + T.page_size - 1) / T.page_size;
         ok = len >= 0 && held >= 0 && held <= T.width && pages <= T.width && t0 + (long long)cnt <= P.tokens;
+        // tokens that go to pages held already: nobody else may hold those (a sequence can be cut back into pages it shares)
+        for (int j = len / T.page_size; ok && cnt && j < min(held, (int)pages); ++j) {
+            const int page = T.block_table[(size_t)s * T.bt_stride + j];
+            ok = page >= 0 && page < T.num_pages && T.refs[page] == 1;
+        }
         want = ok && pages > held ? min((int)pages - held, left + 1) : 0;
     }
     const int p0 = block_scan(want, sums, &npage);
@@ -260,10 +263,11 @@ __global__ void __launch_bounds__(kBookThreads) reserve_kernel(const __grid_cons
     for (int e = i; e < taken; e += kBookThreads) {
         const int o = owner_of(page_s, P.n, e);
         const int page = T.free_list[left - 1 - e];
-        if (page < 0 || page >= T.num_pages) { atomicOr(T.counters + 1, EXL3_PAGES_BAD); continue; }
+        const bool there = page >= 0 && page < T.num_pages;
+        if (!there) atomicOr(T.counters + 1, EXL3_PAGES_BAD);
         if (held_s[o] < 0) continue;
-        T.block_table[(size_t)seq_s[o] * T.bt_stride + held_s[o] + (e - page_s[o])] = page;
-        T.refs[page] = 1;
+        T.block_table[(size_t)seq_s[o] * T.bt_stride + held_s[o] + (e - page_s[o])] = there ? page : -1;
+        if (there) T.refs[page] = 1;
     }
     for (int t = i; t < P.tokens; t += kBookThreads) {
         long long slot = -1, pos = 0;
@@ -485,7 +489,8 @@ extern "C" int exl3_cache_fork(const exl3_page_pools *pools, const exl3_page_tab
     if (rc == EXL3_OK) rc = read_pools(pools, L, G);
     if (rc != EXL3_OK) return rc;
     if (!parents || !children) return EXL3_E_NULL;
-    if (n < 0 || n > kMaxCall) return EXL3_E_SHAPE;
+    if (n < 0 || n > kMaxCall || (long long)G.heads * P.t.page_size * (G.row_bytes >> 4) > INT_MAX - (1 << 16))    // pieces of a page
+        return EXL3_E_SHAPE;
     if (!aligned(parents, 4) || !aligned(children, 4)) return EXL3_E_ALIGN;
     if (n == 0) return EXL3_OK;
     if (!workspace || workspace_bytes < exl3_cache_fork_workspace_bytes(n)) return EXL3_E_WORKSPACE;
@@ -540,7 +545,7 @@ extern "C" int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_t
     int rc = read_tables(tables, P.t);
     if (rc == EXL3_OK) rc = read_pools(pools, L, G);
     if (rc != EXL3_OK) return rc;
-    if (!seqs || !base || !drafts || !path || !taken) return EXL3_E_NULL;
+    if (!seqs || !base || !drafts || (!path && most) || !taken) return EXL3_E_NULL;
     if (n < 0 || n > kMaxCall || most < 0 || most > EXL3_TREE_MAX_DRAFTS || path_stride < most) return EXL3_E_SHAPE;
     if (!aligned(seqs, 4) || !aligned(base, 4) || !aligned(drafts, 4) || !aligned(path, 4) || !aligned(taken, 4)) return EXL3_E_ALIGN;
     if (n == 0) return EXL3_OK;

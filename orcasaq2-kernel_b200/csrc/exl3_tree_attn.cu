@@ -277,7 +277,8 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned *const status = &g_tree_status;
     if (s32(smem) & 1023u) {
-        if (tid == 0) atomicOr(status, 2u);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (tid == 0) { atomicOr(status, 2u); P.joins[blockIdx.x] = make_int4(-1, 0, 0, 0); }
         return;
     }
 
@@ -1032,6 +1033,8 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
         max_drafts < 1 || max_drafts > EXL3_TREE_MAX_DRAFTS ||
         (long long)batch * kvh * (((long long)table_width * cache->page_size + kTok - 1) / kTok + 1) > INT_MAX)
         return EXL3_E_SHAPE;
+    const float s2 = scale * cache->k_scale * 1.4426950408889634f;
+    if (!(fabsf(s2) <= 3e38f)) return EXL3_E_SHAPE;
     if (q_heads / kvh > 2 * kMaxTiles) return EXL3_E_UNSUPPORTED;      // 64 drafts of as many heads are kMaxTiles tiles
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(starts, 4) ||
         !aligned(mask, 8))
@@ -1048,7 +1051,6 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     P.mask = (const long long *)mask;
     P.bt_stride = table_stride; P.width = table_width; P.num_pages = cache->num_pages; P.page_size = cache->page_size;
     P.batch = batch; P.tokens = tokens; P.max_drafts = max_drafts; P.kvh = kvh; P.G = q_heads / kvh; P.tiles = z.tiles;
-    const float s2 = scale * cache->k_scale * 1.4426950408889634f;
     P.negate = s2 < 0.f;
     P.scale_log2 = fmaxf(P.negate ? -s2 : s2, 1e-37f);       // (zero times the minus infinity of an unseen token would be NaN)
     P.v_scale = cache->v_scale;

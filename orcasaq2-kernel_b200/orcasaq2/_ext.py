@@ -837,7 +837,7 @@ def _pools(pools, layout: str, idx: int, num_pages: int):
     if isinstance(pools, torch.Tensor):
         _need(pools.dim() == 5 and pools.get_device() == idx, "pools must be [n, pages, ...] on the device of the tables, or a list of pools")
         shape, stride, size = pools.shape, pools.stride(), pools.element_size()
-        n, step, shape, stride = shape[0], stride[0] * size, shape[1:], stride[1:]
+        n, step, shape, stride = shape[0], stride[0] * size if shape[0] > 1 else 0, shape[1:], stride[1:]
         _need(n <= 1 or step > 0, "pools must be different pools")
         where = ctypes.c_void_p(pools.data_ptr())
     else:
