@@ -650,7 +650,7 @@ def _need(ok: bool, what: str):
 _PACK_CACHE = struct.Struct("@PPqqqiiiiiff").pack
 _PACK_TABLES = struct.Struct("@PPPPPPiiiii").pack
 _PACK_POOLS = struct.Struct("@Pqqqiii4xq").pack
-_I32, _I64 = torch.int32, torch.int64
+_I32, _I64, _Tensor = torch.int32, torch.int64, torch.Tensor
 
 
 def _call(idx: int, fn, *args):
@@ -664,11 +664,19 @@ def _call(idx: int, fn, *args):
         _check(rc, fn.__name__)
 
 
-def _ints(t, name: str, idx: int, dtype=_I32, dim: int = 1):
-    if not isinstance(t, torch.Tensor) or t.get_device() != idx or t.dtype is not dtype or t.dim() != dim or \
-            (t.stride(-1) != 1 and t.shape[-1] > 1):
-        raise RuntimeError(f"{name} must be a {dim}-D {dtype} tensor on CUDA device {idx} with contiguous rows")
-    return t.data_ptr()
+def _ints(t, name: str, idx: int, dtype=_I32):
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.dim() == 1 and t.get_device() == idx and t.is_contiguous():
+        return t.data_ptr()
+    raise RuntimeError(f"{name} must be a contiguous 1-D {dtype} tensor on CUDA device {idx}")
+
+
+def _int_rows(t, name: str, idx: int):
+    """(address, rows, columns, distance of rows)"""
+    if isinstance(t, _Tensor) and t.dtype is _I32 and t.dim() == 2 and t.get_device() == idx:
+        (rows, cols), (step, one) = t.shape, t.stride()
+        if one == 1 or cols <= 1:
+            return t.data_ptr(), rows, cols, step if rows > 1 else cols
+    raise RuntimeError(f"{name} must be a 2-D int32 tensor on CUDA device {idx} with contiguous rows")
 
 
 def _paged(name: str, x: torch.Tensor, k, v, layout: str, k_scale: float, v_scale: float):
@@ -718,9 +726,10 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.
     place in qkv; returns them."""
     cache, kvh, hd = _paged("qk_norm_rope_append", qkv, k_pages, v_pages, layout, k_scale, v_scale)
     idx, dt = qkv.get_device(), qkv.dtype
-    _need(qkv.dim() == 2 and qkv.stride(1) == 1 and q_heads > 0 and qkv.shape[1] >= (q_heads + 2 * kvh) * hd,
+    _need(qkv.dim() == 2, "qk_norm_rope_append: qkv must be [T, (q_heads + 2 kv_heads) * hd] with contiguous rows")
+    (T, wide), (step, one) = qkv.shape, qkv.stride()
+    _need(one == 1 and q_heads > 0 and wide >= (q_heads + 2 * kvh) * hd,
           "qk_norm_rope_append: qkv must be [T, (q_heads + 2 kv_heads) * hd] with contiguous rows")
-    T, wide = qkv.shape
     pos, slot = _ints(positions, "positions", idx, _I64), _ints(slots, "slots", idx, _I64)
     _need(positions.shape[0] == T and slots.shape[0] == T, "qk_norm_rope_append: positions and slots must be [T]")
     cp = sp = qw = kw = None
@@ -748,10 +757,10 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.
               "qk_norm_rope_append: q_out must be [T, q_heads, hd] in the type of qkv, with contiguous heads")
         ldq, qp = q_out.stride(0) if T > 1 else q_heads * hd, q_out.data_ptr()
     if T:
-        _call(idx, lib().exl3_qk_norm_rope_append, qkv.data_ptr(), qkv.stride(0) if T > 1 else -(-wide // 8) * 8, qp, ldq, qw, kw,
+        _call(idx, lib().exl3_qk_norm_rope_append, qkv.data_ptr(), step if T > 1 else -(-wide // 8) * 8, qp, ldq, qw, kw,
               0 if eps is None else 1, 0.0 if eps is None else eps, cp, sp, rot, 1 if interleaved else 0, rows, pos, slot, T,
               q_heads, 1 if dt is torch.bfloat16 else 0, cache)
-    return q_out if q_out is not None else torch.as_strided(qkv, (T, q_heads, hd), (qkv.stride(0), hd, 1))
+    return q_out if q_out is not None else torch.as_strided(qkv, (T, q_heads, hd), (step, hd, 1))
 
 
 def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
@@ -769,31 +778,34 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     not read, those of `out` not written.  Returns [T, q_heads, hd] in q's type."""
     cache, kvh, hd = _paged("tree_attn_paged", q, k_pages, v_pages, layout, k_scale, v_scale)
     idx, dt = q.get_device(), q.dtype
-    _need(q.dim() == 3 and q.shape[2] == hd and q.stride(2) == 1 and (q.shape[1] == 1 or q.stride(1) == hd),
-          "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
-    T, qh, _ = q.shape
-    table, lens, first = _ints(block_table, "block_table", idx, _I32, 2), _ints(seq_lens, "seq_lens", idx), _ints(starts, "starts", idx)
-    B, width = block_table.shape
+    _need(q.dim() == 3, "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
+    (T, qh, last), (step, head, one) = q.shape, q.stride()
+    _need(last == hd and one == 1 and (qh == 1 or head == hd), "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
+    table, B, width, table_step = _int_rows(block_table, "block_table", idx)
+    lens, first = _ints(seq_lens, "seq_lens", idx), _ints(starts, "starts", idx)
     _need(seq_lens.shape[0] == B and starts.shape[0] == B + 1, "tree_attn_paged: seq_lens must be [B], starts [B + 1]")
     mask = None
     if tree_mask is not None:
         mask = _ints(tree_mask, "tree_mask", idx, _I64)
         _need(tree_mask.shape[0] == T, "tree_attn_paged: tree_mask must be [T]")
+    row = qh * hd
+    out_step = row
     if out is None:
-        out = torch.empty((T, qh, hd), dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _need(isinstance(out, torch.Tensor) and out.get_device() == idx and out.dtype is dt and out.shape == q.shape and
               out.stride(2) == 1 and (qh == 1 or out.stride(1) == hd),
               "tree_attn_paged: out must be [T, heads, hd] in the type of q, with contiguous heads")
+        if T > 1:
+            out_step = out.stride(0)
     if T == 0 or B == 0:
         _need(1 <= max_drafts <= TREE_MAX_DRAFTS and qh > 0 and qh % kvh == 0, "tree_attn_paged: bad max_drafts or heads")
         return out
-    L, row = lib(), qh * hd
+    L = lib()
     need = L.exl3_tree_attn_workspace_bytes(B, qh, max_drafts, cache)
-    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
-    _call(idx, L.exl3_tree_attn, q.data_ptr(), q.stride(0) if T > 1 else row, out.data_ptr(), out.stride(0) if T > 1 else row,
-          table, block_table.stride(0) if B > 1 else width, width, lens, first, mask, B, T, max_drafts, qh,
-          hd ** -0.5 if scale is None else scale, 1 if dt is torch.bfloat16 else 0, cache,
+    ws = q.new_empty(need // 2) if need else None         # (a multiple of 16 bytes)
+    _call(idx, L.exl3_tree_attn, q.data_ptr(), step if T > 1 else row, out.data_ptr(), out_step, table, table_step, width, lens,
+          first, mask, B, T, max_drafts, qh, hd ** -0.5 if scale is None else scale, 1 if dt is torch.bfloat16 else 0, cache,
           None if ws is None else ws.data_ptr(), need)
     return out
 
@@ -823,12 +835,13 @@ def _tables(tables: dict, page_size: int):
     if not isinstance(bt, torch.Tensor) or not bt.is_cuda:
         raise RuntimeError("block_table must be a CUDA tensor (this build has no CPU path)")
     idx = bt.get_device()
-    p = (_ints(bt, "block_table", idx, _I32, 2), _ints(lens, "seq_lens", idx), _ints(held, "held", idx),
-         _ints(refs, "refs", idx), _ints(free, "free_list", idx), _ints(cnt, "counters", idx))
-    (S, P), N = bt.shape, refs.shape[0]
+    table, S, P, step = _int_rows(bt, "block_table", idx)
+    p = (_ints(lens, "seq_lens", idx), _ints(held, "held", idx), _ints(refs, "refs", idx), _ints(free, "free_list", idx),
+         _ints(cnt, "counters", idx))
+    N = refs.shape[0]
     if lens.shape[0] != S or held.shape[0] != S or free.shape[0] != N or cnt.shape[0] != 2:
         raise RuntimeError("page tables: seq_lens and held must be [max_seqs], free_list [num_pages], counters [2]")
-    return idx, N, _PACK_TABLES(*p, bt.stride(0) if S > 1 else P, P, S, N, page_size)
+    return idx, N, _PACK_TABLES(table, *p, step, P, S, N, page_size)
 
 
 def _pools(pools, layout: str, idx: int, num_pages: int):
@@ -874,7 +887,7 @@ def cache_fork(pools, tables: dict, parents: torch.Tensor, children: torch.Tenso
         return
     L = lib()
     need = L.exl3_cache_fork_workspace_bytes(n)
-    ws = torch.empty((need,), dtype=torch.uint8, device=parents.device) if need else None
+    ws = parents.new_empty(need // 4) if need else None   # (a multiple of 8 bytes)
     _call(idx, L.exl3_cache_fork, pl, tab, par, kid, n, None if ws is None else ws.data_ptr(), need)
 
 
@@ -888,10 +901,8 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
     n = seqs.shape[0]
     _need(counts.shape[0] == n and n > 0 and tokens >= 0, "cache_reserve: seqs and counts must be [n], n > 0")
-    where = torch.empty((2, tokens), dtype=_I64, device=seqs.device)
-    rows = torch.empty((2 * n + 1,), dtype=_I32, device=seqs.device)
-    slots, positions = where.unbind(0)
-    starts, base = rows.split((n + 1, n))
+    slots = seqs.new_empty(tokens, dtype=_I64)            # (four allocations cost the host less than views of one)
+    positions, starts, base = torch.empty_like(slots), seqs.new_empty(n + 1), torch.empty_like(seqs)
     _call(idx, lib().exl3_cache_reserve, tab, seq, cnt, n, slots.data_ptr(), positions.data_ptr(), tokens, starts.data_ptr(),
           base.data_ptr())
     return slots, positions, starts, base
@@ -904,14 +915,13 @@ def cache_accept(pools, tables: dict, seqs: torch.Tensor, base: torch.Tensor, dr
     to base + taken.  Pages stay with the sequence.  pools, tables: as for cache_fork."""
     idx, pages, tab = _tables(tables, _page_size(pools, layout))
     keep, pl = _pools(pools, layout, idx, pages)
-    p = (_ints(seqs, "seqs", idx), _ints(base, "base", idx), _ints(drafts, "drafts", idx), _ints(path, "path", idx, _I32, 2),
-         _ints(taken, "taken", idx))
-    n, most = path.shape
+    p = (_ints(seqs, "seqs", idx), _ints(base, "base", idx), _ints(drafts, "drafts", idx), _ints(taken, "taken", idx))
+    steps, n, most, step = _int_rows(path, "path", idx)
     _need(seqs.shape[0] == n and base.shape[0] == n and drafts.shape[0] == n and taken.shape[0] == n,
           "cache_accept: seqs, base, drafts and taken must be [n], path [n, most]")
     if n == 0:
         return
-    _call(idx, lib().exl3_cache_accept, pl, tab, p[0], p[1], p[2], p[3], path.stride(0) if n > 1 else most, most, p[4], n)
+    _call(idx, lib().exl3_cache_accept, pl, tab, p[0], p[1], p[2], steps, step, most, p[3], n)
 
 
 def cache_free(tables: dict, seqs: torch.Tensor) -> None:
