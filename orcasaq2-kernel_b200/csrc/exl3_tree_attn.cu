@@ -30,7 +30,17 @@
 // e4m3 caches: a pair of warps per stage fetches the 16 KB of rows into the stage's upper half and widens them in place,
 // from the front, exactly to the 16-bit type of q in the swizzled places; the scales fold into the softmax scale and the
 // normalisation.  (One warp alone needs ten cycles for a conversion of two values that four warps of a scheduler finish
-// in two.)
+// in two.  The selections that keep the two halves of a row's lanes off each other's banks cost as much as the conflicts;
+// bytes fetched to registers instead, all or half of them ahead of the stage's release, took 80 and 75 us for 73.)
+//
+// Measured (24 query / 4 KV heads of 256 unless said): 64 sequences x 16 drafts over 1000 .. 8192 tokens 250 us, 4.9 TB/s
+// (the kernel without products and softmax: 209; HBM's time 190); 61 drafts over 32768 tokens, three tiles, 75 us, 650
+// TFLOP/s (60 without products and softmax); 32 x 8 drafts, e4m3, 71 us (55); 16 sequences of 1 .. 64 drafts, bf16, 32 / 8
+// heads of 128, 117 us (78); 5 drafts over 300 tokens 15 us.  So what bounds it away from HBM's rate is the ring: 160 KB a
+// CTA, a stage's round trip 3 to 3.7 thousand cycles (issue 1.0 to 1.9, arrival 1.0 to 1.3, pick-up and release 0.5), with
+// start-up, join and launches 12 us.  Not kept: two warps a stage for 16-bit caches (75 -> 76 us), three softmax groups at 128
+// dimensions (117 -> 121), V's halves given back one by one (73 -> 80 for e4m3), the first queries loaded by the softmax
+// warps (75.0 -> 74.4, but 71.6 -> 73.1 for e4m3).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -89,7 +99,7 @@ struct Shared {
     };
     int first_seq, first_off;
 };
-static_assert(sizeof(Shared) <= 3072, "shared state");
+static_assert(sizeof(Shared) <= 3 * 1024, "shared state");
 
 template <bool FP8, int HD>
 struct Cfg {
