@@ -19,7 +19,10 @@
 // of one sequence walk the same blocks at the same time and share them in L2.
 // Work is split evenly whatever the lengths: the blocks of all (sequence, KV head) pairs form one line, every CTA
 // takes an equal piece of it (found from the lengths on the device), and a pair that several CTAs share leaves partial
-// sums with their maximum, which a second kernel joins in order (fixed order: the same bytes every run).
+// sums with their maximum, which a second kernel joins in order (fixed order: the same bytes every run).  The change from
+// one pair to the next costs a CTA 8 to 14 thousand cycles (the last products, the result out, new queries in), as much as
+// two to five blocks, so that many empty places follow each pair's blocks on the line (without them the CTA with the most
+// pairs ended 13 to 37 % after the others).
 // The running maximum is only raised when it grows by more than 8 (a factor of 256 that the fp32 sums and the 16-bit
 // probabilities hold easily), so O is seldom rescaled.
 //
@@ -61,6 +64,7 @@ constexpr int kM = 128;                       // rows of a tile
 constexpr int kTok = 128;                     // tokens of a block
 constexpr int kDims = 128;                    // dimensions of a stage
 constexpr int kStageBytes = kTok * kDims * 2; // 32 KB
+constexpr int kMostChange = 8;
 constexpr int kMaxTiles = 16;
 constexpr int kMaxGrid = 148;
 constexpr float kRaise = 8.f;                 // log2 units the maximum may lag behind
@@ -77,6 +81,7 @@ struct Params {
     const long long *mask;
     int bt_stride, width, num_pages, page_size;
     int batch, tokens, max_drafts, kvh, G, tiles;    // tiles: of the sequence with the most drafts
+    int change;                               // places on the line behind a pair's blocks
     float scale_log2, v_scale;
     int negate;                               // the scale is negative: Q K^T is negated, scale_log2 is its size
     int rows_ws;                              // rows of a partial result (a multiple of 32)
@@ -118,6 +123,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool real)
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {      // (without a size: a fifth quicker out of L2)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint32_t pick(bool which, uint32_t a, uint32_t b) {      // (left to itself, the compiler branches)
+    uint32_t v;
+    asm("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tselp.b32 %0, %1, %2, p;\n\t}" : "=r"(v) : "r"(a), "r"(b), "r"((int)which));
+    return v;
 }
 // This thread's arrival on the barrier once its copies so far have landed.
 __device__ __forceinline__ void arrive_behind_copies(uint32_t bar) {
@@ -175,7 +185,7 @@ __device__ __forceinline__ void take_over(int id) { asm volatile("bar.sync %0, 6
 __device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 9, 256;" ::: "memory"); }
 
 // ---------------------------------------------------------------- the line of blocks
-struct Seq { int first, n, len, rows, blocks; };    // first row of q, drafts, tokens, query rows per KV head, blocks
+struct Seq { int first, n, len, rows, blocks, units; };    // first row of q, drafts, tokens, query rows per KV head, blocks, places on the line
 
 __device__ __forceinline__ Seq seq_of(const Params &P, int b) {
     Seq s;
@@ -185,6 +195,7 @@ __device__ __forceinline__ Seq seq_of(const Params &P, int b) {
     s.len = max(0, min(__ldg(P.seq_lens + b), P.width * P.page_size));
     s.rows = min(s.n, P.max_drafts) * P.G;
     s.blocks = s.rows ? max(1, (s.len + kTok - 1) / kTok) : 0;
+    s.units = s.rows ? s.blocks + P.change : 0;
     return s;
 }
 
@@ -199,16 +210,22 @@ struct Walk {
         if (left > 0) s = seq_of(P, b);
     }
     __device__ __forceinline__ bool next() {
-        if (left <= 0) return false;
         for (;;) {
-            nblk = s.rows > kM * m ? s.blocks : 0;
-            if (off < nblk * P.kvh) break;
-            off -= nblk * P.kvh;
-            if (++b >= P.batch) { left = 0; return false; }
-            s = seq_of(P, b);
+            if (left <= 0) return false;
+            const int units = s.rows > kM * m ? s.units : 0;
+            if (off < units * P.kvh) {
+                hk = off / units;
+                blk = off - hk * units;
+                nblk = s.blocks;
+                if (blk < nblk) break;
+                off += units - blk;
+                left -= units - blk;
+            } else {
+                off -= units * P.kvh;
+                if (++b >= P.batch) { left = 0; return false; }
+                s = seq_of(P, b);
+            }
         }
-        hk = off / nblk;
-        blk = off - hk * nblk;
         nb = min(nblk - blk, left);
         off += nb;
         left -= nb;
@@ -316,8 +333,8 @@ tree_attn_kernel(const __grid_constant__ Params P) {
     Seq s0 = {};
     if (b0 < b1) s0 = seq_of(P, b0);
     const auto blocks_of = [&](int m) {                      // of the run, in tile m
-        int v = s0.rows > kM * m ? s0.blocks * P.kvh : 0;
-        for (int b = b0 + 1; b < b1; ++b) { const Seq s = seq_of(P, b); v += s.rows > kM * m ? s.blocks * P.kvh : 0; }
+        int v = s0.rows > kM * m ? s0.units * P.kvh : 0;
+        for (int b = b0 + 1; b < b1; ++b) { const Seq s = seq_of(P, b); v += s.rows > kM * m ? s.units * P.kvh : 0; }
         return v;
     };
     for (int t = 0; t < P.tiles; ++t) {
@@ -360,7 +377,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
         if (off >= 0 && off < v) {
             int b = b0;
             for (Seq s = s0;; s = seq_of(P, b)) {
-                const int n = s.rows > kM * m ? s.blocks * P.kvh : 0;
+                const int n = s.rows > kM * m ? s.units * P.kvh : 0;
                 if (off < n) break;
                 off -= n;
                 ++b;
@@ -880,10 +897,10 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                     const uint32_t at0 = tall ? tall_at[0] : wide_at[0] + part * 2048, at1 = tall ? tall_at[1] : wide_at[1] + part * 2048;
                     const auto write = [&](const uint4 &v, uint32_t to) {
                         uint4 one, two;
-                        widen4<T>(swap ? v.z : v.x, one.x, one.y);
-                        widen4<T>(swap ? v.w : v.y, one.z, one.w);
-                        widen4<T>(swap ? v.x : v.z, two.x, two.y);
-                        widen4<T>(swap ? v.y : v.w, two.z, two.w);
+                        widen4<T>(pick(swap, v.z, v.x), one.x, one.y);
+                        widen4<T>(pick(swap, v.w, v.y), one.z, one.w);
+                        widen4<T>(pick(swap, v.x, v.z), two.x, two.y);
+                        widen4<T>(pick(swap, v.y, v.w), two.z, two.w);
                         *reinterpret_cast<uint4 *>(dst + to) = one;
                         *reinterpret_cast<uint4 *>(dst + (to ^ 16)) = two;
                     };
@@ -1041,7 +1058,7 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
         table_stride < table_width || (long long)table_width * cache->page_size > INT_MAX - 1024 || (q_stride & 7) ||
         (out_stride & 7) || q_stride < (long long)q_heads * hd || out_stride < (long long)q_heads * hd ||
         max_drafts < 1 || max_drafts > EXL3_TREE_MAX_DRAFTS ||
-        (long long)batch * kvh * (((long long)table_width * cache->page_size + kTok - 1) / kTok + 1) > INT_MAX)
+        (long long)batch * kvh * (((long long)table_width * cache->page_size + kTok - 1) / kTok + 1 + kMostChange) > INT_MAX)
         return EXL3_E_SHAPE;
     const float s2 = scale * cache->k_scale * 1.4426950408889634f;
     if (!(fabsf(s2) <= 3e38f)) return EXL3_E_SHAPE;
@@ -1064,6 +1081,10 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     P.negate = s2 < 0.f;
     P.scale_log2 = fmaxf(P.negate ? -s2 : s2, 1e-37f);       // (zero times the minus infinity of an unseen token would be NaN)
     P.v_scale = cache->v_scale;
+    // Measured (us, with 0 / 1 / 2 / 3 / 4 places): 64 x 16 drafts 253 / 240 / 233 / 229 / 230, 61 drafts over 32768 tokens 80 / 79 /
+    // 76 / 73 / 73, e4m3 71 / 60 / 59.5 / 60 / 62; 128 dimensions with 0 / 3 / 5 / 6 / 8: 127 / 107 / 100 / 102 / 106, e4m3 146 /
+    // 124 / 119 / 120 / 122.
+    P.change = hd == 128 ? 5 : cache->dtype == EXL3_KV_E4M3 ? 2 : 3;
     P.rows_ws = z.rows_ws;
     P.joins = (int4 *)workspace;
     P.part_ml = (float *)((char *)workspace + z.joins);
