@@ -32,18 +32,18 @@
 //
 // e4m3 caches: a pair of warps per stage fetches the 16 KB of rows into the stage's upper half and widens them in place,
 // from the front, exactly to the 16-bit type of q in the swizzled places; the scales fold into the softmax scale and the
-// normalisation.  (One warp alone needs ten cycles for a conversion of two values that four warps of a scheduler finish
-// in two.  The selections that keep the two halves of a row's lanes off each other's banks cost as much as the conflicts;
-// bytes fetched to registers instead, all or half of them ahead of the stage's release, took 80 and 75 us for 73.)
+// normalisation.  The selections that keep the two halves of a row's lanes off each other's banks are worth it (60 against
+// 63 us with the conflicts); bytes fetched to registers instead, all or half of them ahead of the stage's release, took 80 and
+// 75 us when this took 73.
 //
-// Measured (24 query / 4 KV heads of 256 unless said): 64 sequences x 16 drafts over 1000 .. 8192 tokens 250 us, 4.9 TB/s
-// (the kernel without products and softmax: 209; HBM's time 190); 61 drafts over 32768 tokens, three tiles, 75 us, 650
-// TFLOP/s (60 without products and softmax); 32 x 8 drafts, e4m3, 71 us (55); 16 sequences of 1 .. 64 drafts, bf16, 32 / 8
-// heads of 128, 117 us (78); 5 drafts over 300 tokens 15 us.  So what bounds it away from HBM's rate is the ring: 160 KB a
-// CTA, a stage's round trip 3 to 3.7 thousand cycles (issue 1.0 to 1.9, arrival 1.0 to 1.3, pick-up and release 0.5), with
-// start-up, join and launches 12 us.  Not kept: two warps a stage for 16-bit caches (75 -> 76 us), three softmax groups at 128
-// dimensions (117 -> 121), V's halves given back one by one (73 -> 80 for e4m3), the first queries loaded by the softmax
-// warps (75.0 -> 74.4, but 71.6 -> 73.1 for e4m3).
+// Measured (device time, 24 query / 4 KV heads of 256 unless said; the GPUs differ by some per cent): 64 sequences x 16 drafts
+// over 1000 .. 8192 tokens 220 to 250 us, 5.6 TB/s (the kernel without products and softmax: 214; HBM's time 190); 61 drafts
+// over 32768 tokens, three tiles, 69 to 77 us, 714 TFLOP/s (58 without products and softmax); 32 x 8 drafts, e4m3, 57 us (52);
+// 16 sequences of 1 .. 64 drafts, bf16, 32 / 8 heads of 128, 95 to 109 us (77); 5 drafts over 300 tokens 15 us (12).  So what
+// bounds it away from HBM's rate is the ring: 160 KB a CTA, a stage's round trip 3 to 3.7 thousand cycles (issue 1.0 to 1.9,
+// arrival 1.0 to 1.3, pick-up and release 0.5), with start-up, join and launches 12 us.  Not kept: two warps a stage for
+// 16-bit caches (77 -> 81 us, 248 -> 243), three softmax groups at 128 dimensions (117 -> 121), the next stage's lines asked
+// into L2 (+ 5 to 15 %), the queries loaded by the softmax warps (15.4 -> 14.7, but 248 -> 251 at the largest).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -477,20 +477,25 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                         const int buf = cnt % C::kBufs;
                         // before V(i) lies K(i + 1), before V(0) also K(0)
                         stage = (stage + (i + 1 < wk.nb ? H : 0) + (i ? 0 : H)) % C::kStages;
-                        int st = stage;
-                        for (int h = 0; h < H && ok; ++h) {
-                            ok = mbar_wait(s32(&S.v_full[st]), phases >> st & 1, status);
+                        // e4m3: V's halves are used and given back as they come (57 against 60 us; 16 bits: 79 against 77), but where
+                        // drafts are looked over (`clean`) all of V has to be there before P is.
+                        const int early = !FP8 || H == 1 || (wk.blk + i + 1) * kTok > wk.s.len - wk.s.n ? H : 1;
+                        int st = stage, got = 0;
+                        const auto here = [&] {
+                            const bool is = mbar_wait(s32(&S.v_full[st]), phases >> st & 1, status);
                             phases ^= 1u << st;
                             if (++st == C::kStages) st = 0;
-                        }
-                        if (!ok) break;
-                        mbar_arrive(s32(&S.v_here[buf]));
-                        ok = mbar_wait(s32(&S.p_ready[buf]), cnt / C::kBufs & 1, status);
+                            if (++got == H) mbar_arrive(s32(&S.v_here[buf]));
+                            return is;
+                        };
+                        while (ok && got < early) ok = here();
+                        if (ok) ok = mbar_wait(s32(&S.p_ready[buf]), cnt / C::kBufs & 1, status);
                         if (ok && i == 0 && wk.index) ok = mbar_wait(s32(&S.o_free), (wk.index - 1) & 1, status);
-                        if (!ok) break;
-                        if constexpr (!FP8) fence_async();
-                        fence_after_sync();
-                        for (int h = 0; h < H; ++h) {
+                        for (int h = 0; h < H && ok; ++h) {
+                            if (got == h) ok = here();
+                            if (!ok) break;
+                            if constexpr (!FP8) fence_async();
+                            fence_after_sync();
                             const uint64_t vd = vdesc + (uint32_t)(stage * (kStageBytes >> 4));
                             const uint32_t p = tmem + HD + buf * kTok + h * 32;
 #pragma unroll
@@ -499,7 +504,7 @@ tree_attn_kernel(const __grid_constant__ Params P) {
                             umma_commit(s32(&S.empty[stage]));
                             if (++stage == C::kStages) stage = 0;
                         }
-                        umma_commit(s32(&S.pv_done[buf]));
+                        if (ok) umma_commit(s32(&S.pv_done[buf]));
                     }
                 }
                 umma_commit(s32(&S.drain[1]));
