@@ -896,7 +896,7 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     seq_lens.  Returns (slots [tokens], positions [tokens], starts [n + 1], base [n]): where each new token goes and its
     position, one sequence after the other, the sequences' first rows (what qk_norm_rope_append and tree_attn_paged
     take), and the lengths before.  Slots behind the last token, and those of a sequence that could not be served
-    (counters[1]), are -1."""
+    (counters[1]: too few pages, or its next tokens would lie on a page that another sequence holds too), are -1."""
     idx, _, tab = _tables(tables, page_size)
     seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
     n = seqs.shape[0]
