@@ -19,7 +19,7 @@ inline int integer_k(int k_times_2) {
 
 // Launch with programmatic stream serialization: the grid may be scheduled while its predecessor on
 // the stream is still running; the kernel itself waits (griddepcontrol.wait) before it touches
-// anything the predecessor produces.
+// anything the predecessor produces.  A launch that is refused leaves no error behind for the next call to find.
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
                               Args &&...args) {
@@ -33,7 +33,9 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+    if (e != cudaSuccess) cudaGetLastError();
+    return e;
 }
 
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? EXL3_OK : EXL3_E_LAUNCH; }

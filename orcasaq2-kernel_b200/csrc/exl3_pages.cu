@@ -373,6 +373,7 @@ struct AcceptParams {
 // rows is a chain of four dependent loads, so a CTA does it once for several pools, and reads the next pool's rows while
 // it writes one's (64 sequences in 64 layers: 30 us, 4.8 TB/s; a CTA per pool took 40 us).
 constexpr int kAcceptThreads = 128;
+constexpr int kMaxRowBytes = 1024;
 __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_constant__ AcceptParams P,
                                                                 const __grid_constant__ PoolList L,
                                                                 const __grid_constant__ RowGeom G) {
@@ -456,10 +457,27 @@ static int read_tables(const exl3_page_tables *in, Tables &t) {
     return EXL3_OK;
 }
 
+// The most shared memory that a call of accept_kernel can ask for, allowed once per device whatever the call's own size: beside
+// the kernel's 1 KB of static shared memory a launch is refused from 47 KB on, and a limit set call by call could be lowered by
+// another thread between this one's setting and its launch.
+static bool allow_accept_rows() {
+    static bool ready[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && ready[dev]) return true;
+    if (cudaFuncSetAttribute(accept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * EXL3_TREE_MAX_DRAFTS * kMaxRowBytes) !=
+        cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+    return true;
+}
+
 static int read_pools(const exl3_page_pools *in, PoolList &l, RowGeom &g) {
     if (!in || !in->pools) return EXL3_E_NULL;
     if (in->num_pools <= 0 || in->num_pools > EXL3_PAGES_MAX_POOLS || in->heads <= 0 || in->row_bytes <= 0 || (in->row_bytes & 15) ||
-        in->row_bytes > 1024 || in->heads > 65535 || in->page_stride <= 0 || in->head_stride < in->row_bytes ||
+        in->row_bytes > kMaxRowBytes || in->heads > 65535 || in->page_stride <= 0 || in->head_stride < in->row_bytes ||
         in->token_stride < in->row_bytes || (in->page_stride & 15) || (in->head_stride & 15) || (in->token_stride & 15))
         return EXL3_E_SHAPE;
     if (in->pool_stride < 0 || (in->pool_stride & 15)) return EXL3_E_SHAPE;
@@ -557,9 +575,7 @@ extern "C" int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_t
     if (P.heads < 1) P.heads = 1;
     if (P.heads > G.heads) P.heads = G.heads;
     const int smem = 2 * P.heads * per_head;
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(accept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return EXL3_E_LAUNCH;
+    if (!allow_accept_rows()) return EXL3_E_LAUNCH;
     const int groups = (G.heads + P.heads - 1) / P.heads;
     P.pools = pools->num_pools;
     P.per = (int)((long long)n * P.pools * groups / (2 * 7 * 148));
