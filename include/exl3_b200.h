@@ -465,7 +465,8 @@ int exl3_cache_reserve(const exl3_page_tables *tables, const void *seqs, const v
  * After a tree of drafts[i] tokens behind base[i] was verified: the rows at base + path[i][j], j < taken[i] (at most
  * `most`, path is int32 [n][path_stride], NULL when most is 0), move to base + j in all pools, and seq_lens[seqs[i]] =
  * base + taken.  The pages stay with the sequence.  The rows are moved as if all were read before the first is written;
- * pages that are written must not be shared.
+ * pages that are written must not be shared.  A sequence is never made longer: base + taken beyond seq_lens is
+ * EXL3_PAGES_BAD, as after an exl3_cache_reserve that could not be served, whose tokens are not there.
  */
 int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_tables *tables, const void *seqs, const void *base,
                       const void *drafts, const void *path, int path_stride, int most, const void *taken, int n,

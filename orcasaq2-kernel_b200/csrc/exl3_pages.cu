@@ -387,7 +387,10 @@ __global__ void __launch_bounds__(kAcceptThreads) accept_kernel(const __grid_con
     bool bad = s < 0 || s >= T.max_seqs || base < 0 || drafts < 0 || taken < 0 || taken > P.most || taken > drafts;
     if (!bad) {
         const int held = T.held[s];
-        bad = held > T.width || (long long)base + drafts > (long long)held * T.page_size;
+        // never longer than it is: behind its end lies nothing when the reserve before was refused.  (The CTA that writes the new
+        // length, base + taken, may have done so already: that passes too, and where it does not pass nobody writes.)
+        const int len = *(volatile const int *)(T.seq_lens + s);
+        bad = held > T.width || (long long)base + drafts > (long long)held * T.page_size || (long long)base + taken > len;
         for (int j = tid; j < b; j += kAcceptThreads) bad |= P.seqs[j] == s;    // the same sequence twice: the first counts
         if (!bad && tid < taken) {
             const int from = P.path[(size_t)b * P.path_stride + tid];

@@ -912,7 +912,8 @@ def cache_accept(pools, tables: dict, seqs: torch.Tensor, base: torch.Tensor, dr
                  taken: torch.Tensor, layout: str = "HND") -> None:
     """After drafts[i] drafted tokens behind base[i] of sequence seqs[i] were verified: move the rows of the accepted
     drafts path[i, :taken[i]] (int32 [n, most], most <= 64) to base[i], base[i] + 1, .. in every pool, and set seq_lens
-    to base + taken.  Pages stay with the sequence.  pools, tables: as for cache_fork."""
+    to base + taken, which may not be more than it is (a cache_reserve that could not be served gave no rows to take: the
+    sequence stays as it was, counters[1]).  Pages stay with the sequence.  pools, tables: as for cache_fork."""
     idx, pages, tab = _tables(tables, _page_size(pools, layout))
     keep, pl = _pools(pools, layout, idx, pages)
     p = (_ints(seqs, "seqs", idx), _ints(base, "base", idx), _ints(drafts, "drafts", idx), _ints(taken, "taken", idx))
