@@ -454,19 +454,21 @@ int exl3_cache_fork(const exl3_page_pools *pools, const exl3_page_tables *tables
 /*
  * counts[i] more tokens for seqs[i]: pages as needed, seq_lens raised.  Outputs: base int32 [n] (the lengths before),
  * starts int32 [n + 1] (prefix sums of counts), and for the tokens, one sequence after the other, slots and positions
- * int64 [tokens] (what exl3_qk_norm_rope_append takes).  Tokens of a sequence that is not served, and entries behind
- * the last token, have slot -1 (the latter position 0).  tokens: room in the outputs, at most 2^20; a sequence that
- * does not fit is not served, nor is one whose tokens would lie on a page that another sequence holds too (cut back by
- * exl3_cache_accept into pages that it shares).  n >= 1.
+ * int64 [tokens], as exl3_qk_norm_rope_append takes them.  Positions are base + 0, 1, ..: right for prompts and chains of
+ * drafts; a draft in a tree is rotated for base + its depth, which the caller has to put there.  Tokens of a sequence that
+ * is not served, and entries behind the last token, have slot -1 (the latter position 0).  tokens: room in the outputs, at
+ * most 2^20; a sequence that does not fit is not served, nor is one whose tokens would lie on a page that another sequence
+ * holds too (cut back by exl3_cache_accept into pages that it shares).  n >= 1.
  */
 int exl3_cache_reserve(const exl3_page_tables *tables, const void *seqs, const void *counts, int n, void *slots,
                        void *positions, int tokens, void *starts, void *base, void *stream);
 /*
  * After a tree of drafts[i] tokens behind base[i] was verified: the rows at base + path[i][j], j < taken[i] (at most
  * `most`, path is int32 [n][path_stride], NULL when most is 0), move to base + j in all pools, and seq_lens[seqs[i]] =
- * base + taken.  The pages stay with the sequence.  The rows are moved as if all were read before the first is written;
- * pages that are written must not be shared.  A sequence is never made longer: base + taken beyond seq_lens is
- * EXL3_PAGES_BAD, as after an exl3_cache_reserve that could not be served, whose tokens are not there.
+ * base + taken.  Keys are moved as they are: with keys rotated for base + depth, path[i] goes from a root of the tree down.
+ * The pages stay with the sequence.  The rows are moved as if all were read before the first is written; pages that are
+ * written must not be shared.  A sequence is never made longer: base + taken beyond seq_lens is EXL3_PAGES_BAD, as after
+ * an exl3_cache_reserve that could not be served, whose tokens are not there.
  */
 int exl3_cache_accept(const exl3_page_pools *pools, const exl3_page_tables *tables, const void *seqs, const void *base,
                       const void *drafts, const void *path, int path_stride, int most, const void *taken, int n,

@@ -895,7 +895,8 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     """Room for counts[i] more tokens of sequence seqs[i] (int32 [n], 1 <= n <= 1024): takes pages as needed and raises
     seq_lens.  Returns (slots [tokens], positions [tokens], starts [n + 1], base [n]): where each new token goes and its
     position, one sequence after the other, the sequences' first rows (what qk_norm_rope_append and tree_attn_paged
-    take), and the lengths before.  Slots behind the last token, and those of a sequence that could not be served
+    take), and the lengths before.  Positions are base + 0, 1, ..: right for prompts and chains; a draft in a tree is rotated
+    for base + its depth, so add depth - place to them first.  Slots behind the last token, and those of a sequence that could not be served
     (counters[1]: too few pages, or its next tokens would lie on a page that another sequence holds too), are -1."""
     idx, _, tab = _tables(tables, page_size)
     seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
