@@ -35,7 +35,7 @@ struct AppendParams {
     long long page_stride, head_stride, tok_stride;
     long long total_slots;
     int page_size;
-    float k_inv_scale, v_inv_scale;
+    float k_scale, v_scale;              // e4m3 pools hold value / scale
 };
 
 constexpr int kAppendWarps = 8;
@@ -53,11 +53,13 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return lo | hi << 16;
 }
 
+// e4m3: the quotient itself (times the reciprocal, values at the border between two e4m3 numbers went to the wrong one, and a
+// scale below 2^-128 has no reciprocal).
 template <typename T, bool FP8>
-__device__ __forceinline__ void store8(void *base, long long off, const float2 (&f)[4], float inv_scale) {
+__device__ __forceinline__ void store8(void *base, long long off, const float2 (&f)[4], float scale) {
     if constexpr (FP8) {
-        const uint2 r = make_uint2(e4m3x4(f[0].x * inv_scale, f[0].y * inv_scale, f[1].x * inv_scale, f[1].y * inv_scale),
-                                   e4m3x4(f[2].x * inv_scale, f[2].y * inv_scale, f[3].x * inv_scale, f[3].y * inv_scale));
+        const uint2 r = make_uint2(e4m3x4(f[0].x / scale, f[0].y / scale, f[1].x / scale, f[1].y / scale),
+                                   e4m3x4(f[2].x / scale, f[2].y / scale, f[3].x / scale, f[3].y / scale));
         *reinterpret_cast<uint2 *>(static_cast<unsigned char *>(base) + off) = r;
     } else {
         const uint4 r = make_uint4(Type16<T>::pack(f[0].x, f[0].y), Type16<T>::pack(f[1].x, f[1].y),
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_token_kernel(const _
             if (h >= P.qh + P.kvh) {                                 // value head
                 if (!slot_ok) continue;
                 const long long to = dst_off + (h - P.qh - P.kvh) * P.head_stride;
-                if constexpr (FP8) store8<T, true>(P.v, to, y, P.v_inv_scale);
+                if constexpr (FP8) store8<T, true>(P.v, to, y, P.v_scale);
                 else *reinterpret_cast<uint4 *>(static_cast<T *>(P.v) + to) = x[j];
                 continue;
             }
@@ -201,7 +203,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_token_kernel(const _
             if (is_q)
                 store8<T, false>(P.q_out, (long long)t * P.ld_q + (long long)h * HD + 8 * l, y, 1.f);
             else
-                store8<T, FP8>(P.k, dst_off + (h - P.qh) * P.head_stride, y, P.k_inv_scale);
+                store8<T, FP8>(P.k, dst_off + (h - P.qh) * P.head_stride, y, P.k_scale);
         }
     }
 }
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_stream_kernel(con
                 if constexpr (FP8) {
                     float2 y[4];
                     unpack8<T>(x[j], y);
-                    store8<T, true>(P.v, dst_off + h * P.head_stride, y, P.v_inv_scale);
+                    store8<T, true>(P.v, dst_off + h * P.head_stride, y, P.v_scale);
                 } else {
                     *reinterpret_cast<uint4 *>(static_cast<T *>(P.v) + dst_off + h * P.head_stride) = x[j];
                 }
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_stream_kernel(con
             if (kind == 0)
                 store8<T, false>(P.q_out, (long long)t * P.ld_q + (long long)h * HD + 8 * l, y, 1.f);
             else
-                store8<T, FP8>(P.k, dst_off + h * P.head_stride, y, P.k_inv_scale);
+                store8<T, FP8>(P.k, dst_off + h * P.head_stride, y, P.k_scale);
         }
     }
 }
@@ -375,7 +377,7 @@ extern "C" int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out
     P.page_stride = cache->page_stride; P.head_stride = cache->head_stride; P.tok_stride = cache->token_stride;
     P.page_size = cache->page_size;
     P.total_slots = (long long)cache->num_pages * cache->page_size;
-    P.k_inv_scale = 1.f / cache->k_scale; P.v_inv_scale = 1.f / cache->v_scale;
+    P.k_scale = cache->k_scale; P.v_scale = cache->v_scale;
     const bool fp8 = cache->dtype == EXL3_KV_E4M3, adj = interleaved != 0;
     cudaStream_t st = (cudaStream_t)stream;
     cudaError_t e;
