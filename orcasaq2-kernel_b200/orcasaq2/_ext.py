@@ -674,9 +674,9 @@ def _int_rows(t, name: str, idx: int):
     """(address, rows, columns, distance of rows)"""
     if isinstance(t, _Tensor) and t.dtype is _I32 and t.dim() == 2 and t.get_device() == idx:
         (rows, cols), (step, one) = t.shape, t.stride()
-        if one == 1 or cols <= 1:
+        if (one == 1 or cols <= 1) and (rows <= 1 or step < 1 << 31):          # (the C entry points take the distance in 32 bits)
             return t.data_ptr(), rows, cols, step if rows > 1 else cols
-    raise RuntimeError(f"{name} must be a 2-D int32 tensor on CUDA device {idx} with contiguous rows")
+    raise RuntimeError(f"{name} must be a 2-D int32 tensor on CUDA device {idx} with contiguous rows less than 2^31 apart")
 
 
 def _paged(name: str, x: torch.Tensor, k, v, layout: str, k_scale: float, v_scale: float):
@@ -781,6 +781,7 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _need(q.dim() == 3, "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
     (T, qh, last), (step, head, one) = q.shape, q.stride()
     _need(last == hd and one == 1 and (qh == 1 or head == hd), "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
+    _need(1 <= max_drafts <= TREE_MAX_DRAFTS, f"tree_attn_paged: max_drafts must be 1 .. {TREE_MAX_DRAFTS}")
     table, B, width, table_step = _int_rows(block_table, "block_table", idx)
     lens, first = _ints(seq_lens, "seq_lens", idx), _ints(starts, "starts", idx)
     _need(seq_lens.shape[0] == B and starts.shape[0] == B + 1, "tree_attn_paged: seq_lens must be [B], starts [B + 1]")
@@ -799,7 +800,7 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if T > 1:
             out_step = out.stride(0)
     if T == 0 or B == 0:
-        _need(1 <= max_drafts <= TREE_MAX_DRAFTS and qh > 0 and qh % kvh == 0, "tree_attn_paged: bad max_drafts or heads")
+        _need(qh > 0 and qh % kvh == 0, "tree_attn_paged: bad heads")
         return out
     L = lib()
     need = L.exl3_tree_attn_workspace_bytes(B, qh, max_drafts, cache)
@@ -901,7 +902,8 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     idx, _, tab = _tables(tables, page_size)
     seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
     n = seqs.shape[0]
-    _need(counts.shape[0] == n and n > 0 and tokens >= 0, "cache_reserve: seqs and counts must be [n], n > 0")
+    _need(counts.shape[0] == n and n > 0, "cache_reserve: seqs and counts must be [n], n > 0")
+    _need(0 <= tokens <= 1 << 20, "cache_reserve: tokens must be 0 .. 2^20")
     slots = seqs.new_empty(tokens, dtype=_I64)            # (four allocations cost the host less than views of one)
     positions, starts, base = torch.empty_like(slots), seqs.new_empty(n + 1), torch.empty_like(seqs)
     _call(idx, lib().exl3_cache_reserve, tab, seq, cnt, n, slots.data_ptr(), positions.data_ptr(), tokens, starts.data_ptr(),
