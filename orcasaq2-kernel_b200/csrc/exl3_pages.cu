@@ -5,8 +5,9 @@
 // Bookkeeping: `free_list` is a stack of page numbers (counters[0] of them), `refs` counts the sequences that hold a
 // page.  Every call takes or returns pages for all its sequences at once: what sequence i needs is known from its
 // lengths, an exclusive prefix sum over the call gives its place in the stack, and so the result is the one that
-// serving the sequences in the order of the call would give, whatever order the threads run in.  This is a few
-// hundred bytes of work bound by latency: one CTA, one thread per sequence.
+// serving the sequences in the order of the call would give, whatever order the threads run in, with one exception: once
+// the stack is too short for a sequence, none behind it takes pages, though fewer might do for it (its place in the
+// stack lies behind the place of the one that got none).
 // Data: rows (one token of one head) are moved with 16-byte accesses for all pools (K and V of every layer) in one
 // launch; bound by HBM, 2 x the bytes of the rows.
 //

@@ -898,7 +898,8 @@ def cache_reserve(tables: dict, seqs: torch.Tensor, counts: torch.Tensor, page_s
     position, one sequence after the other, the sequences' first rows (what qk_norm_rope_append and tree_attn_paged
     take), and the lengths before.  Positions are base + 0, 1, ..: right for prompts and chains; a draft in a tree is rotated
     for base + its depth, so add depth - place to them first.  Slots behind the last token, and those of a sequence that could not be served
-    (counters[1]: too few pages, or its next tokens would lie on a page that another sequence holds too), are -1."""
+    (counters[1]: too few pages are left for it, or for one before it in the list, behind which none takes pages; or its next
+    tokens would lie on a page that another sequence holds too), are -1."""
     idx, _, tab = _tables(tables, page_size)
     seq, cnt = _ints(seqs, "seqs", idx), _ints(counts, "counts", idx)
     n = seqs.shape[0]
