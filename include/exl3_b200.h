@@ -366,9 +366,11 @@ typedef struct exl3_paged_cache {
  * contiguous cache).  No counterpart in the reference: the serving engine does it there.
  *   qkv       [tokens][ld_qkv] fp16 (bf16 when is_bf16): q_heads, then kv_heads key heads, then kv_heads value heads;
  *             not modified, except the query heads when q_out is NULL (they are then rewritten in place)
- *   q_out     [tokens][ld_q_out] (q_heads * head_dim values per row used), or NULL
+ *   q_out     [tokens][ld_q_out] (q_heads * head_dim values per row used), or NULL; it must not overlap qkv,
+ *             except that it may be the query heads' own place
  *   norm      non-zero: every query and key head is multiplied by rsqrt(mean(x^2) + eps) and by q_weight / k_weight
- *             ([head_dim], the type of qkv; NULL = ones) before it is rotated
+ *             ([head_dim], the type of qkv; NULL = ones) before it is rotated; zero: the weights are not used.  (A norm by
+ *             1 + w takes 1 + w, rounded to that type.)
  *   cos, sin  fp32 [max_pos][rot_dim / 2]; rot_dim a multiple of 16, 0 = no rotation; dimensions from rot_dim on are
  *             not rotated.  interleaved 0: pairs (i, i + rot_dim / 2), else (2 i, 2 i + 1)
  *   positions, slots   int64 [tokens].  slot = page * page_size + offset; a token whose slot lies outside the pool
@@ -389,7 +391,8 @@ int exl3_qk_norm_rope_append(void *qkv, long long ld_qkv, void *q_out, long long
  * is set in mask[i] (its ancestors and itself, in a tree); without a mask it sees the drafts up to itself.  A row
  * that sees nothing yields zeros.  One token per sequence is ordinary decode attention.
  *   q, out       [tokens][q_heads][head_dim] fp16 (bf16 when is_bf16), rows q_stride / out_stride elements apart
- *                (multiples of 8), 16-byte aligned; rows at or behind starts[batch] are neither read nor written
+ *                (multiples of 8), 16-byte aligned; rows at or behind starts[batch] are neither read nor written.  out
+ *                may be q itself (the same address and stride); it must not overlap q otherwise
  *   block_table  int32 [batch][table_stride], table_width entries of a row used: the page of tokens i*page_size ..;
  *                tokens on a page number outside the pool are not visible, entries behind a sequence's length are
  *                not read
@@ -409,8 +412,9 @@ int exl3_tree_attn(const void *q, long long q_stride, void *out, long long out_s
                    int table_stride, int table_width, const void *seq_lens, const void *starts, const void *mask,
                    int batch, int tokens, int max_drafts, int q_heads, float scale, int is_bf16,
                    const exl3_paged_cache *cache, void *workspace, size_t workspace_bytes, void *stream);
-/* Sticky status word of exl3_tree_attn's bounded waits on the current device (0 = none ran out; waits for the device),
- * its reset, and the self-test of the wait as for exl3_gemm_tc. */
+/* Sticky status word of exl3_tree_attn's bounded waits on the current device (0 = none ran out; waits for the device):
+ * non-zero means that the output of some call since the last reset is not valid.  Its reset, and the self-test of the wait
+ * as for exl3_gemm_tc. */
 int exl3_tree_attn_status(unsigned *status_out);
 int exl3_tree_attn_status_reset(void);
 int exl3_tree_attn_selftest_wait(unsigned limit_us, void *stream);
@@ -425,8 +429,10 @@ int exl3_tree_attn_selftest_wait(unsigned limit_us, void *stream);
  * Lists of sequence numbers (int32, device memory) have at most EXL3_PAGES_MAX_SEQS entries.  The result is the one
  * of serving the entries in their order, except that once the stack is too short for one, none behind it takes pages.
  * An entry that cannot be served leaves its sequence as it was and sets a status bit (sticky; the caller reads and
- * clears it when it likes): EXL3_PAGES_EXHAUSTED when the stack has too few pages, EXL3_PAGES_BAD when an index, a
- * length or the state does not allow it (a sequence twice in a call, ...).
+ * clears it when it likes): EXL3_PAGES_EXHAUSTED when the stack has too few pages, EXL3_PAGES_BAD when an index or a
+ * length does not allow it (a sequence twice in a call, ...).  EXL3_PAGES_BAD also reports a broken state, a page number
+ * outside the pool in the stack or in a table: an entry that meets one is served all the same, with page -1 there, which
+ * holds no tokens (no slots, not visible to the attention); the caller gives such a sequence up.
  * Data is moved in all pools of `exl3_page_pools` (K and V of every layer: equal layouts, strides and row size in
  * bytes, multiples of 16; page p of a pool and page p of another belong together).
  */

@@ -717,7 +717,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor | None, sin: torch.
     """Norms of the query and key heads, rotary embedding and the append to a paged cache, one pass over
     qkv [T, >= (q_heads + 2 kv_heads) * hd] (fp16 or bf16, contiguous rows; hd 128 or 256).
 
-    Every query and key head is normed (x * rsqrt(mean(x^2) + eps) * weight; eps None: not, weight None: ones) and
+    Every query and key head is normed (x * rsqrt(mean(x^2) + eps) * weight; eps None: not, nor weighted; weight None: ones) and
     rotated by row positions[t] of cos, sin (fp32 [max_pos, rot / 2], rot a multiple of 16; None: not rotated; pairs
     (i, i + rot/2), or (2i, 2i + 1) when interleaved).  Keys and values go to slots[t] = page * page_size + offset of
     the page pools (see decode_attn_paged; any page size), as value / scale in float8_e4m3fn ones; a slot outside the
@@ -775,7 +775,8 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     whose bit j is set in tree_mask[row] (int64 [T]: its ancestors and itself; None: every draft up to itself).  A row
     that sees nothing gives zeros.  Page pools and block_table as for decode_attn_paged (q's type or float8_e4m3fn; page
     size a multiple of 16); tokens on a page number outside the pool are not visible.  Rows of q from starts[B] on are
-    not read, those of `out` not written.  Returns [T, q_heads, hd] in q's type."""
+    not read, those of `out` not written; `out` may be q itself.  Returns [T, q_heads, hd] in q's type; not valid when a
+    bounded wait ran out meanwhile, which tree_attn_status() tells."""
     cache, kvh, hd = _paged("tree_attn_paged", q, k_pages, v_pages, layout, k_scale, v_scale)
     idx, dt = q.get_device(), q.dtype
     _need(q.dim() == 3, "tree_attn_paged: q must be [T, heads, hd] with contiguous heads")
@@ -812,7 +813,8 @@ def tree_attn_paged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
 
 def tree_attn_status(device: torch.device) -> int:
-    """Sticky status word of tree_attn_paged's bounded waits on `device` (0 = healthy)."""
+    """Sticky status word of tree_attn_paged's bounded waits on `device`, which it waits for (0 = healthy; else the output of
+    some call is not valid)."""
     word = ctypes.c_uint(0)
     with torch.cuda.device(device):
         _check(lib().exl3_tree_attn_status(ctypes.byref(word)), "exl3_tree_attn_status")
