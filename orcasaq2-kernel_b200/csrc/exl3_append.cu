@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_stream_kernel(con
 template <typename T, bool FP8, int HD>
 static cudaError_t launch_append(const AppendParams &P, bool adjacent, cudaStream_t st) {
     // Measured with 24 / 4 heads of 256 (us, a CTA per token against a warp per token): 4.2 / 10.4 at 5 tokens, 10.7 / 11.7 at
-    // 1024 into an e4m3 cache, 14.3 / 14.4 at 1024 and 24.6 / 20.6 at 2048 into an fp16 one, 163 / 100 at 16384.
+    // 1024 into an e4m3 cache, 14.3 / 14.4 at 1024 and 24.6 / 20.6 at 2048 into an fp16 one, 163 / 100 at 16384.  The crossing
+    // lies at about 1024 for 16-bit caches and somewhat above for e4m3 ones, where the one threshold for both costs up to 1 us.
     if (P.tokens <= kFewTokens) {
         auto kernel = adjacent ? append_token_kernel<T, FP8, HD, true> : append_token_kernel<T, FP8, HD, false>;
         return launch_pdl(kernel, dim3(P.tokens), dim3(kAppendWarps * 32), 0, st, P);

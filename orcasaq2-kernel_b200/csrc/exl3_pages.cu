@@ -7,9 +7,12 @@
 // lengths, an exclusive prefix sum over the call gives its place in the stack, and so the result is the one that
 // serving the sequences in the order of the call would give, whatever order the threads run in, with one exception: once
 // the stack is too short for a sequence, none behind it takes pages, though fewer might do for it (its place in the
-// stack lies behind the place of the one that got none).
+// stack lies behind the place of the one that got none).  For fork and reserve this is a few hundred bytes of work bound
+// by latency: one CTA, one thread per sequence.  free passes four times over every entry of its sequences' rows of the
+// table in that one CTA: 9 us for 64 pages in all, 62 us for 64 sequences of 256, 481 us for 64 of 2048.
 // Data: rows (one token of one head) are moved with 16-byte accesses for all pools (K and V of every layer) in one
-// launch; bound by HBM, 2 x the bytes of the rows.
+// launch; bound by HBM: the rows are written once per child and read once per parent (its children's CTAs find them in
+// L2).  Sixteen parents' partial pages for 96 children, 482 MB written, 80 read: 125 us, what a plain fill of 482 MB takes.
 //
 // What cannot be served is not an error of the call (the host does not wait for it): a sequence for which no pages
 // are left, or whose arguments do not fit its state, stays as it was and a bit of counters[1] is set.

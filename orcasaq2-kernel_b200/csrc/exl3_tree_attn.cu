@@ -34,13 +34,14 @@
 // from the front, exactly to the 16-bit type of q in the swizzled places; the scales fold into the softmax scale and the
 // normalisation.  The selections that keep the two halves of a row's lanes off each other's banks are worth it (60 against
 // 63 us with the conflicts); bytes fetched to registers instead, all or half of them ahead of the stage's release, took 80 and
-// 75 us when this took 73.
+// 75 us at a time when this took 73 (57 now).
 //
 // Measured (device time, 24 query / 4 KV heads of 256 unless said; the GPUs differ by some per cent): 64 sequences x 16 drafts
-// over 1000 .. 8192 tokens 220 to 250 us, 5.6 TB/s (the kernel without products and softmax: 214; HBM's time 190); 61 drafts
+// over 1000 .. 8192 tokens 220 to 250 us, 5.6 to 4.9 TB/s (the kernel without products and softmax: 214; HBM's time 190); 61 drafts
 // over 32768 tokens, three tiles, 69 to 77 us, 714 TFLOP/s (58 without products and softmax); 32 x 8 drafts, e4m3, 57 us (52);
 // 16 sequences of 1 .. 64 drafts, bf16, 32 / 8 heads of 128, 95 to 109 us (77); 5 drafts over 300 tokens 15 us (12).  So what
-// bounds it away from HBM's rate is the ring: 160 KB a CTA, a stage's round trip 3 to 3.7 thousand cycles (issue 1.0 to 1.9,
+// bounds it away from HBM's rate is the ring: five stages, 160 KB a CTA (beside 128 dimensions, where the queries take 32 KB and not
+// 64, a sixth would fit a CTA of the 16-bit caches; not measured), a stage's round trip 3 to 3.7 thousand cycles (issue 1.0 to 1.9,
 // arrival 1.0 to 1.3, pick-up and release 0.5), with start-up, join and launches 12 us.  Not kept: two warps a stage for
 // 16-bit caches (77 -> 81 us, 248 -> 243), three softmax groups at 128 dimensions (117 -> 121), the next stage's lines asked
 // into L2 (+ 5 to 15 %), the queries loaded by the softmax warps (15.4 -> 14.7, but 248 -> 251 at the largest).
@@ -64,7 +65,7 @@ constexpr int kM = 128;                       // rows of a tile
 constexpr int kTok = 128;                     // tokens of a block
 constexpr int kDims = 128;                    // dimensions of a stage
 constexpr int kStageBytes = kTok * kDims * 2; // 32 KB
-constexpr int kMostChange = 8;
+constexpr int kMostChange = 5;                // the largest Params::change
 constexpr int kMaxTiles = 16;
 constexpr int kMaxGrid = 148;
 constexpr float kRaise = 8.f;                 // log2 units the maximum may lag behind
@@ -1089,7 +1090,7 @@ extern "C" int exl3_tree_attn(const void *q, long long q_stride, void *out, long
     // Measured (us, with 0 / 1 / 2 / 3 / 4 places): 64 x 16 drafts 253 / 240 / 233 / 229 / 230, 61 drafts over 32768 tokens 80 / 79 /
     // 76 / 73 / 73, e4m3 71 / 60 / 59.5 / 60 / 62; 128 dimensions with 0 / 3 / 5 / 6 / 8: 127 / 107 / 100 / 102 / 106, e4m3 146 /
     // 124 / 119 / 120 / 122.
-    P.change = hd == 128 ? 5 : cache->dtype == EXL3_KV_E4M3 ? 2 : 3;
+    P.change = hd == 128 ? kMostChange : cache->dtype == EXL3_KV_E4M3 ? 2 : 3;
     P.rows_ws = z.rows_ws;
     P.joins = (int4 *)workspace;
     P.part_ml = (float *)((char *)workspace + z.joins);
